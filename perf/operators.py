@@ -1,0 +1,411 @@
+"""The norm in front of a projection, microscaled 4-bit (MXFP4) quantisation, and projections on an MXFP4 base, as timing cases.
+
+Three operators and the run of them together, over the sizes of the benchmark layer (hidden 4096, intermediate 12288, heads of
+128) and of the tensor-parallel shards of the 72B-class layer (hidden 8192, 29568 intermediate):
+
+  norm      residual addition, root-mean-square norm, output as bf16 and, where asked, as e4m3 codes with one scale per row
+  quantize  a tensor to e2m1 codes with one power-of-two scale per 32 elements, and the values those codes stand for
+  project   y = x_q W_q^T (both MXFP4) + every tenant's LoRA term, x quantised on the way, with the fused neighbours
+  block     the norm's MXFP4 codes given to the projection behind it
+
+`run` computes them in plain torch operations, or through the package's entry points where `own` is set.  Batches of up to
+256 tokens are then replayed from a CUDA graph, as serving engines do; larger ones are called.
+"""
+import math
+
+import torch
+
+own = False
+
+DEV = "cuda"
+MAX_M = 8192              # the engine's most tokens per forward
+GRAPH_M = 256
+EPS = 1e-6
+SHAPES = {                # name -> (input features, widths of the merged outputs)
+    "qkv": (4096, (4096, 1024, 1024)),
+    "o": (4096, (4096,)),
+    "gate_up": (4096, (12288, 12288)),
+    "down": (12288, (4096,)),
+    "tp8_qkv": (8192, (1024, 128, 128)),          # one rank of eight of the 72B-class layer
+    "tp8_gate_up": (8192, (3696, 3696)),
+    "tp4_down": (7392, (8192,)),                  # one of four: its input features are no multiple of 256
+}
+
+
+def _norm(tokens, K, heads=1, residual=True, quant="fp8"):
+    return {"kind": "norm", "tokens": tokens, "heads": heads, "K": K, "residual": residual, "quant": quant}
+
+
+def _quantize(rows, K):
+    return {"kind": "quantize", "rows": rows, "K": K}
+
+
+def _project(shape, tokens, batch, adapters="bf16", tenants=32, rank=64, silu=False, residual=False):
+    return {"kind": "project", "shape": shape, "tokens": tokens, "batch": batch, "adapters": adapters, "tenants": tenants,
+            "rank": rank, "silu": silu, "residual": residual}
+
+
+def listed():
+    return [
+        # the norm before a projection in a decode step: 16 sequences, latency is all
+        dict(_norm(16, 4096), name="norm_decode"),
+        # the same norm of the largest forward
+        dict(_norm(8192, 4096), name="norm_prefill"),
+        # queries' norm per head of 128, read where the merged projection left them
+        dict(_norm(2001, 128, heads=32, residual=False, quant=""), name="norm_heads"),
+        # a ragged batch of activations on its way into the down projection
+        dict(_quantize(333, 12288), name="quantize_activations"),
+        # a weight quantised when it is loaded
+        dict(_quantize(24576, 4096), name="quantize_weight"),
+        # one user typing: the smallest call
+        dict(_project("o", 1, "decode", tenants=8), name="project_one_token"),
+        # an odd number of running sequences, adapters kept in FP8 to fit more of them
+        dict(_project("qkv", 23, "decode", adapters="fp8"), name="project_decode_fp8_adapters"),
+        # a full decode batch on the widest projection, an adapter of its own for nearly every sequence
+        dict(_project("gate_up", 32, "decode"), name="project_decode"),
+        # prompts of several tenants of rank 16, ragged size, input features that end inside a 256-element block
+        dict(_project("tp4_down", 777, "prefill", tenants=4, rank=16), name="project_ragged"),
+        # the down projection with the activation before it and the residual stream behind it
+        dict(_project("down", 2048, "prefill", silu=True, residual=True), name="project_down_fused"),
+        # the largest forward of the widest projection
+        dict(_project("gate_up", 8192, "prefill"), name="project_largest"),
+        # half a decoder layer's front: residual and norm, codes handed on, merged projection
+        {"kind": "block", "shape": "qkv", "tokens": 48, "batch": "decode", "adapters": "bf16", "tenants": 16, "rank": 32,
+         "silu": False, "residual": False, "name": "block_decode"},
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi + 0.49)))))))
+
+
+def draw(rng):
+    kind = rng.choice(["norm", "norm", "quantize", "project", "project", "project", "block"])
+    if kind == "norm":
+        if rng.random() < 0.3:
+            return _norm(_log_int(rng, 1, 4096), rng.choice([64, 128, 256]), heads=rng.choice([1, 5, 8, 32]), residual=False, quant="")
+        quant = rng.choice(["fp8", "fp8", ""])
+        K = _log_int(rng, 7, 12288) if rng.random() < 0.3 else 16 * _log_int(rng, 4, 768)
+        return _norm(_log_int(rng, 1, MAX_M), K, residual=rng.random() < 0.7, quant=quant)
+    if kind == "quantize":
+        K = 32 * _log_int(rng, 1, 400)
+        return _quantize(_log_int(rng, 1, max(2, 24576 * 4096 // K)), K)
+    shape, rank, tenants = rng.choice(sorted(SHAPES)), rng.choice([16, 32, 64, 64, 128]), rng.choice([1, 3, 4, 8, 16, 32])
+    batch = rng.choice(["decode", "mixed", "prefill", "prefill"])
+    tokens = _log_int(rng, 1, 256) if batch == "decode" else _log_int(rng, 33, 512) if batch == "mixed" else _log_int(rng, 64, 2048)
+    down = shape.endswith("down")
+    if kind == "block" and not down:
+        return dict(_project(shape, tokens, batch, tenants=tenants, rank=rank), kind="block")
+    return _project(shape, tokens, batch, adapters=rng.choice(["bf16", "bf16", "fp8", "nvfp4"]), tenants=tenants, rank=rank,
+                    silu=down and rng.random() < 0.5, residual=(down or shape == "o") and rng.random() < 0.5)
+
+
+# ---------------------------------------------------------------------------------------------------------------- inputs
+def _gen(seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed * 7919 + 11)
+    return g
+
+
+def _randn(g, *shape):
+    return torch.randn(*shape, generator=g, device=DEV)
+
+
+def _activations(g, rows, K):
+    """bf16 rows of unit variance with a few channels eight times as large, as a decoder's residual stream has them."""
+    x = _randn(g, rows, K)
+    x[:, :: max(1, K // 7)] *= 8.0
+    return x.to(torch.bfloat16)
+
+
+def _zipf_counts(tokens, tenants):
+    share = 1.0 / torch.arange(1, tenants + 1, dtype=torch.float64) ** 1.1
+    want = share / share.sum() * tokens
+    counts = want.floor().long()
+    counts[torch.argsort(want - counts, descending=True)[: tokens - int(counts.sum())]] += 1
+    return counts
+
+
+def _slot_ids(case, seed):
+    """Adapter slot of every token (-1: none).  decode: a slot per sequence, one in sixteen without; prefill: prompts of
+    contiguous tokens whose sizes follow Zipf(1.1) over the tenants; mixed: 32 decoding sequences and pieces of two prompts."""
+    M, L, g = case["tokens"], case["tenants"], torch.Generator().manual_seed(seed)
+    if case["batch"] == "prefill":
+        return torch.repeat_interleave(torch.randperm(L, generator=g), _zipf_counts(M, L)[torch.randperm(L, generator=g)])
+    n = M if case["batch"] == "decode" else min(32, M)
+    ids = torch.randint(0, L, (n,), generator=g)
+    ids[torch.rand(n, generator=g) < 1.0 / 16] = -1
+    a, b = int(torch.randint(0, L, (1,), generator=g)), int(torch.randint(0, L, (1,), generator=g))
+    rest = M - n
+    return torch.cat([ids, torch.full((rest - rest // 4,), a), torch.full((rest // 4,), b)])
+
+
+def _distinct(case):
+    """Tenants that have a token, on average."""
+    L, M = case["tenants"], case["tokens"]
+    if case["batch"] == "prefill":
+        return int((_zipf_counts(M, L) > 0).sum())
+    n = M if case["batch"] == "decode" else min(32, M)
+    return min(L, L * (1.0 - (1.0 - 1.0 / L) ** n) + (2 if M > n else 0))
+
+
+def _meta(ids, L):
+    """vLLM's five metadata tensors of a batch, as the serving engine keeps them."""
+    ids = ids.to(torch.int32)
+    seg_n, seg_start, seg_ids = torch.zeros(L + 1, dtype=torch.int32), torch.zeros(L + 2, dtype=torch.int32), torch.full((L + 1,), -1, dtype=torch.int32)
+    if bool((ids >= 0).any()):
+        uniq, counts = torch.unique(ids, sorted=True, return_counts=True)
+        seg_n[: len(uniq)], seg_ids[: len(uniq)] = counts.to(torch.int32), uniq
+        seg_start[1: len(uniq) + 1] = torch.cumsum(counts, 0).to(torch.int32)
+    return tuple(t.to(DEV) for t in (ids, torch.argsort(ids, stable=True).to(torch.int32), seg_n, seg_start, seg_ids))
+
+
+def _graphed(call, keep):
+    """`call` captured in a CUDA graph: a function that replays it and gives the outputs of the capture."""
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+
+    def replay():
+        graph.replay()
+        return out
+
+    replay.keep = (graph, keep)
+    return replay
+
+
+def prepare(case, seed):
+    g = _gen(seed)
+    if case["kind"] == "norm":
+        M, H, K = case["tokens"], case["heads"], case["K"]
+        if H > 1:                                   # the heads lie in a wider row: keys and values follow
+            x = _activations(g, M, (H + 2) * K).view(M, H + 2, K)[:, :H]
+        else:
+            x = _activations(g, M, K)
+        s = {"case": case, "x": x, "w": (1.0 + 0.1 * _randn(g, K)).to(torch.bfloat16)}
+        s["residual"] = (_activations(g, M * H, K) * 3.0).view(x.shape) if case["residual"] else None
+    elif case["kind"] == "quantize":
+        s = {"case": case, "x": _randn(g, case["rows"], case["K"]).mul_(0.02).to(torch.bfloat16)}
+    else:
+        K, widths = SHAPES[case["shape"]]
+        M, N, L, R = case["tokens"], sum(widths), case["tenants"], case["rank"]
+        codes, scales = _mx_quantize(_randn(g, N, K).mul_(0.02))
+        s = {"case": case, "w_codes": codes[:, 0::2] | (codes[:, 1::2] << 4), "w_scales": scales, "ids": _slot_ids(case, seed)}
+        a = [(torch.rand(L, 1, R, K, generator=g, device=DEV) * 2 - 1).div_(math.sqrt(K)).to(torch.bfloat16) for _ in widths]
+        b = [_randn(g, L, 1, n, R).mul_(0.01).to(torch.bfloat16) for n in widths]
+        s |= {"a": a, "b": b, "x": _activations(g, M, K * (2 if case["silu"] else 1)), "meta": _meta(s["ids"], L)}
+        s["slot"] = s["ids"].to(DEV)
+        s["stream"] = _activations(g, M, N) if case["residual"] else None
+        if case["kind"] == "block":
+            s["w"] = (1.0 + 0.1 * _randn(g, K)).to(torch.bfloat16)
+            s["residual"] = _activations(g, M, K) * 3.0
+        # what the adapters' storage stands for: the values a stored adapter multiplies with
+        s["a_values"], s["b_values"] = ([_stored(t, case["adapters"]) for t in ts] for ts in (a, b))
+    if own:
+        s["call"] = _own_call(s)
+        if case.get("tokens", MAX_M) * case.get("heads", 1) <= GRAPH_M:
+            s["call"] = _graphed(s["call"], s)
+    return s
+
+
+def _own_call(s):
+    """The call of the package's entry points that one pass makes."""
+    from onebase_b200.kernels.mxfp4 import dequantize, quantize
+    from onebase_b200.kernels.mxfp4_lora_vllm import VllmFusedMXFP4LoRA
+    from onebase_b200.kernels.rms_norm import rms_norm
+    case = s["case"]
+    if case["kind"] == "norm":
+        x, w, residual, quant = s["x"], s["w"], s["residual"], case["quant"] or None
+
+        def call():
+            r = rms_norm(x, w, EPS, residual=residual, quant=quant)
+            return [t for t in r if t is not None]
+        return call
+    if case["kind"] == "quantize":
+        x = s["x"]
+        return lambda: dequantize(*quantize(x))
+    op = VllmFusedMXFP4LoRA(s["w_codes"], s["w_scales"], tuple(s["a"]), tuple(s["b"]), MAX_M, lora_fmt=case["adapters"])
+    x, meta, silu, stream = s["x"], s["meta"], case["silu"], s["stream"]
+    if case["kind"] == "project":
+        return lambda: op(x, meta, silu_mul=silu, residual=stream)
+    w, residual = s["w"], s["residual"]
+
+    def block():
+        n = rms_norm(x, w, EPS, residual=residual, quant="mxfp4")
+        return n.residual, op(n.y, meta, quantized=(n.codes, n.scales))
+    return block
+
+
+# ------------------------------------------------------------------------------------------------------------ plain forms
+def _e2m1(v):
+    """Code of each value, ties to the even code, saturating at 6 (bit 3 = sign)."""
+    a = v.abs()
+    mag = ((a > 0.25).to(torch.uint8) + (a >= 0.75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) + (a >= 3.5) + (a > 5.0))
+    return mag + (v < 0).to(torch.uint8) * 8
+
+
+def _mx_quantize(x):
+    """fp32 [m, k] -> (e2m1 codes uint8 [m, k], scale bytes uint8 [m, k/32]): 2^(floor(log2 max|block|) - 2), at least 2^-127."""
+    blocks = x.unflatten(-1, (-1, 32))
+    top = blocks.abs().amax(-1)
+    byte = ((top.view(torch.int32) >> 23) - 2).clamp(min=0)
+    codes = _e2m1(blocks * torch.exp2((127 - byte).float()).unsqueeze(-1))
+    return codes.flatten(-2), byte.to(torch.uint8)
+
+
+def _mx_values(codes, scales):
+    """What codes [m, k] and scale bytes [m, k/32] stand for, fp32."""
+    grid = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], device=codes.device)
+    v = grid[(codes & 7).long()] * (1.0 - 2.0 * (codes >> 3).float())
+    return (v.unflatten(-1, (-1, 32)) * torch.exp2(scales.float() - 127.0).unsqueeze(-1)).flatten(-2)
+
+
+def _stored(t, fmt):
+    """The values of an adapter buffer [l, 1, rows, cols] as `fmt` stores it (fp8: a scale per row; nvfp4: e4m3 scales per 16
+    elements and one global per adapter)."""
+    if fmt == "bf16":
+        return t[:, 0]
+    v = t[:, 0].float()
+    if fmt == "fp8":
+        sc = (v.abs().amax(-1, keepdim=True) / 448.0).clamp(min=1e-12)
+        return (v / sc).clamp(-448.0, 448.0).to(torch.float8_e4m3fn).float() * sc
+    gs = (2688.0 / v.abs().amax((1, 2), keepdim=True).clamp(min=1e-12)).unsqueeze(-1)
+    blocks = v.unflatten(-1, (-1, 16))
+    sf = (gs * (blocks.abs().amax(-1, keepdim=True) * (1.0 / 6.0))).clamp(max=448.0).to(torch.float8_e4m3fn).float()
+    codes = _e2m1(blocks * torch.where(sf != 0, 1.0 / (sf * (1.0 / gs)), torch.zeros_like(sf)))
+    grid = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], device=t.device)
+    return (grid[(codes & 7).long()] * (1.0 - 2.0 * (codes >> 3).float()) * (sf / gs)).flatten(-2)
+
+
+def _plain_norm(x, w, residual):
+    t = x.float() if residual is None else x.float() + residual.float()
+    return t, t * torch.rsqrt(t.square().mean(-1, keepdim=True) + EPS) * w.float()
+
+
+def _plain_project(s, xq, x):
+    """xq: the quantised input's values, x: the input itself; both fp32.  Returns bf16."""
+    case = s["case"]
+    packed = s["w_codes"]
+    w = _mx_values(torch.stack((packed & 15, packed >> 4), -1).flatten(-2), s["w_scales"])
+    y = xq @ w.t()
+    M, L, R = case["tokens"], case["tenants"], case["rank"]
+    mine = s["slot"].unsqueeze(1) == torch.arange(L, device=DEV)                      # [M, L]: the token's tenant
+    y += torch.cat([((x @ a.float().reshape(L * R, -1).t()).view(M, L, R) * mine.unsqueeze(-1)).view(M, L * R)
+                    @ b.float().transpose(1, 2).reshape(L * R, -1) for a, b in zip(s["a_values"], s["b_values"])], 1)
+    return (y if s["stream"] is None else y + s["stream"].float()).to(torch.bfloat16)
+
+
+def _plain_input(s):
+    """The projection's input in bf16: silu(gate) * up where the activation is fused, formed as the engine forms it."""
+    x = s["x"]
+    if not s["case"]["silu"]:
+        return x
+    K = x.shape[1] // 2
+    gate = x[:, :K].float()
+    return ((gate / (1.0 + torch.exp(-gate))).to(torch.bfloat16).float() * x[:, K:].float()).to(torch.bfloat16)
+
+
+def run(state):
+    if own:
+        return state["call"]()
+    case = state["case"]
+    if case["kind"] == "norm":
+        t, y = _plain_norm(state["x"], state["w"], state["residual"])
+        out = [y.to(torch.bfloat16)]
+        if case["residual"]:
+            out.append(t.to(torch.bfloat16))
+        if case["quant"]:
+            scale = (y.abs().amax(-1) / 448.0).clamp(min=1.0 / (448.0 * 512.0))
+            out += [(y / scale.unsqueeze(-1)).clamp(-448.0, 448.0).to(torch.float8_e4m3fn), scale]
+        return out
+    if case["kind"] == "quantize":
+        return _mx_values(*_mx_quantize(state["x"].float())).to(torch.bfloat16)
+    if case["kind"] == "project":
+        x = _plain_input(state).float()
+        return _plain_project(state, _mx_values(*_mx_quantize(x)), x)
+    t, y = _plain_norm(state["x"], state["w"], state["residual"])
+    return t.to(torch.bfloat16), _plain_project(state, _mx_values(*_mx_quantize(y)), y.to(torch.bfloat16).float())
+
+
+# --------------------------------------------------------------------------------------------- the same, in 64 bits
+def _exact_mx(x):
+    """Values of x (float64) rounded to MXFP4, block by block of 32: every step exact in 64 bits."""
+    b = x.reshape(x.shape[0], -1, 32)
+    top = b.abs().amax(-1, keepdim=True)
+    unit = torch.exp2((torch.frexp(top).exponent.double() - 3.0).clamp(min=-127.0))
+    q = (b / unit).abs()
+    step = torch.where(q < 2.0, 0.5, torch.where(q < 4.0, 1.0, 2.0)).double()
+    return (torch.minimum(torch.round(q / step) * step, torch.full_like(q, 6.0)) * torch.sign(b) * unit).reshape(x.shape)
+
+
+def _exact_norm(s):
+    t = s["x"].double() if s["residual"] is None else s["x"].double() + s["residual"].double()
+    ms = (t * t).sum(-1, keepdim=True) / t.shape[-1]
+    return t, t / torch.sqrt(ms + EPS) * s["w"].double()
+
+
+def exact(case, seed):
+    global own
+    was, own = own, False
+    try:
+        s = prepare(case, seed)
+    finally:
+        own = was
+    if case["kind"] == "norm":
+        t, y = _exact_norm(s)
+        out = [y] + ([t] if case["residual"] else [])
+        if case["quant"]:
+            scale = (y.abs().amax(-1) / 448.0).clamp(min=1.0 / (448.0 * 512.0))
+            out += [y / scale.unsqueeze(-1), scale]
+        return out
+    if case["kind"] == "quantize":
+        return _exact_mx(s["x"].double())
+    lead = []
+    if case["kind"] == "block":
+        t, y = _exact_norm(s)
+        lead, xq, x = [t], _exact_mx(y), y
+    else:
+        x = s["x"].double()
+        if case["silu"]:
+            K = x.shape[1] // 2
+            x = ((x[:, :K] * torch.sigmoid(x[:, :K])).to(torch.bfloat16).double() * x[:, K:]).to(torch.bfloat16).double()
+        xq = _exact_mx(x)
+    packed = s["w_codes"].long()
+    table = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -0.0, -0.5, -1.0, -1.5, -2.0, -3.0, -4.0, -6.0], dtype=torch.float64, device=DEV)
+    N, K = packed.shape[0], 2 * packed.shape[1]
+    w = torch.empty(N, K, dtype=torch.float64, device=DEV)
+    w[:, 0::2], w[:, 1::2] = table[packed % 16], table[packed // 16]
+    w *= torch.repeat_interleave(torch.exp2(s["w_scales"].double() - 127.0), 32, dim=1)
+    y = xq @ w.t()
+    for tenant in range(case["tenants"]):
+        rows = torch.nonzero(s["slot"] == tenant).flatten()
+        if len(rows):
+            y[rows] += torch.cat([x[rows] @ a[tenant].double().t() @ b[tenant].double().t() for a, b in zip(s["a_values"], s["b_values"])], 1)
+    if s["stream"] is not None:
+        y += s["stream"].double()
+    return tuple(lead + [y]) if lead else y
+
+
+# ------------------------------------------------------------------------------------------------------------------ work
+def work(case):
+    if case["kind"] == "norm":
+        n, K = case["tokens"] * case["heads"], case["K"]
+        per = 2 + 2 + (4 if case["residual"] else 0) + (1 if case["quant"] else 0)
+        return {"bytes": n * K * per + 2 * K + (4 * n if case["quant"] else 0), "flops": 6 * n * K}
+    if case["kind"] == "quantize":
+        return {"bytes": case["rows"] * case["K"] * 4, "flops": 4 * case["rows"] * case["K"]}
+    K, widths = SHAPES[case["shape"]]
+    M, N, S, R = case["tokens"], sum(widths), len(widths), case["rank"]
+    stored = {"bf16": 2.0, "fp8": 1.0, "nvfp4": 0.5625}[case["adapters"]]
+    d = _distinct(case)
+    nbytes = N * K * 17 / 32 + d * R * (S * K + N) * stored + M * K * 2 * (2 if case["silu"] else 1) + M * N * 2 * (2 if case["residual"] else 1)
+    flops = 2.0 * M * N * K + 2.0 * M * R * (S * K + N)
+    if case["kind"] == "block":
+        nbytes += 4 * M * K + 2 * K
+        flops += 6 * M * K
+    return {"bytes": nbytes, "flops": flops}

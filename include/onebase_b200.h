@@ -272,6 +272,48 @@ int ob_requant_fp8_rows(const void* src, int64_t rows, int32_t cols, void* codes
 int ob_requant_nvfp4(const void* src, int32_t l, int32_t rows, int32_t cols, void* packed, void* sf, float* inv_global,
                      void* amax_scratch, void* cuda_stream);
 
+/* Root-mean-square norm of the rows of x, with the residual's addition before it and low-precision codes behind it: what sits in
+ * front of qkv_proj and gate_up_proj in a decoder layer, and, per head, on queries and keys.  Row (m, h), m < M, h < H:
+ *     s = x + residual  (fp32);   residual_out = s;   y = (s * weight) / sqrt(mean(s^2) + eps)
+ * y and residual_out are rounded once, to `dtype`.  `quant` asks for codes of the fp32 y as well, dense at row m * H + h:
+ *     OB_QUANT_FP8     codes [M * H, K] e4m3 with scales [M * H] fp32 = max(max|y| / 448, 1 / (448 * 512)): the layout and the
+ *                      scale's floor of ob_k1_fp8's own quantization
+ *     OB_QUANT_MXFP4   codes [M * H, K/2] and scales [M * H, K/32] as ob_mxfp4_quantize gives them
+ * Strides are in elements: `*_ld` between tokens, `*_hd` between a token's heads (H = 1: unused).  An output may be the same memory as an input of the same strides, else they must not
+ * overlap.  A row that holds a NaN or an infinity has NaN for its scale and codes (and for its y, but for zeros where an infinity divides a
+ * number).  One launch, capturable, no workspace; M = 0 does nothing.  No counterpart in the reference, which leaves the norm to
+ * vLLM (RMSNorm, vllm/model_executor/layers/layernorm.py). */
+enum { OB_QUANT_NONE = 0, OB_QUANT_FP8 = 1, OB_QUANT_MXFP4 = 2 };
+typedef struct ObRmsNorm {
+    int32_t M, H, K;                 /* tokens, heads of a token (1: rows of K), elements of a row; MXFP4: K a multiple of 32 */
+    int32_t dtype;                   /* x, residual, residual_out and y: OB_DTYPE_BF16 or OB_DTYPE_F16 */
+    int32_t weight_dtype;            /* weight: `dtype` or OB_DTYPE_F32 */
+    int32_t quant;                   /* OB_QUANT_* */
+    float eps;                       /* >= 0 */
+    const void* x;
+    int64_t x_ld, x_hd;
+    const void* weight;              /* [K]; null: ones */
+    const void* residual;            /* null: none */
+    int64_t residual_ld, residual_hd;
+    void* residual_out;              /* null: not stored */
+    int64_t residual_out_ld, residual_out_hd;
+    void* y;                         /* null: not stored */
+    int64_t y_ld, y_hd;
+    void* codes;
+    void* scales;
+} ObRmsNorm;
+int ob_rms_norm(const ObRmsNorm* norm, void* cuda_stream);
+
+/* MXFP4 (OCP microscaling): e2m1 elements, packed two per byte along K (element 2i in the low nibble), one power-of-two scale per 32
+ * of them, stored as exponent + 127.  The scale of a block is 2^(floor(log2 max|x|) - 2), an element the e2m1 value next to x / scale
+ * (ties to even, saturating at 6); a block that holds a NaN or an infinity gets scale byte 255, the format's NaN.  x is
+ * [rows, K] of `dtype` (BF16, F16 or F32), rows ldx elements apart, K a multiple of 32; codes [rows, K/2] and scales [rows, K/32] are dense.
+ * rows = 0 does nothing.  No counterpart in the reference (its 4-bit base is NVFP4). */
+int ob_mxfp4_quantize(const void* x, int32_t dtype, int64_t rows, int32_t K, int64_t ldx, void* codes, void* scales, void* cuda_stream);
+/* The values codes and scales stand for, as `dtype`, rows ldo elements apart (rounded once where `dtype` does not hold one). */
+int ob_mxfp4_dequantize(const void* codes, const void* scales, int32_t dtype, int64_t rows, int32_t K, void* out, int64_t ldo,
+                        void* cuda_stream);
+
 /* Token sort + segment index on the device: vLLM's LoRAKernelMeta.prepare_tensors
  * (vllm/lora/ops/triton_ops/lora_kernel_metadata.py:110-168) incl. its stale-on-no-adapter behaviour.
  * token_lora [M] int32 in; the five metadata tensors out (tok/srt of capacity >= M, seg_* of L+1 / L+2 / L+1). */
@@ -292,7 +334,7 @@ int ob_segment_index(const int32_t* token_lora, int32_t M, int32_t L, int32_t* t
  * then zero their buffers together before the next call.  Plain peer loads and stores only (no multicast, no TMA). */
 #define OB_MAX_RANKS 8
 #define OB_IPC_HANDLE_BYTES 64
-enum { OB_DTYPE_BF16 = 0, OB_DTYPE_F32 = 1 };
+enum { OB_DTYPE_BF16 = 0, OB_DTYPE_F32 = 1, OB_DTYPE_F16 = 2 };   /* (the all-reduce serves BF16 and F32) */
 enum { OB_AR_AUTO = 0, OB_AR_ONE_SHOT = 1, OB_AR_TWO_SHOT = 2 };   /* auto: two shots above 512 KB on more than 2 ranks */
 typedef struct ObComm {
     int32_t world, rank;             /* 2..OB_MAX_RANKS ranks */

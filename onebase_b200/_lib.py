@@ -51,7 +51,8 @@ class ObWorkspaceShape(C.Structure):
 
 
 OB_MAX_RANKS = 8
-OB_DTYPE_BF16, OB_DTYPE_F32 = 0, 1
+OB_DTYPE_BF16, OB_DTYPE_F32, OB_DTYPE_F16 = 0, 1, 2
+OB_QUANT_NONE, OB_QUANT_FP8, OB_QUANT_MXFP4 = 0, 1, 2
 OB_AR_AUTO, OB_AR_ONE_SHOT, OB_AR_TWO_SHOT = 0, 1, 2
 
 
@@ -62,6 +63,15 @@ class ObComm(C.Structure):
 class ObTileCfg(C.Structure):
     _fields_ = [("tn", C.c_int32), ("split2", C.c_int32), ("split1", C.c_int32), ("stages", C.c_int32),
                 ("wait_ms", C.c_int32), ("fused", C.c_int32), ("prefill", C.c_int32), ("stream", C.c_int32)]
+
+
+class ObRmsNorm(C.Structure):
+    _fields_ = [("M", C.c_int32), ("H", C.c_int32), ("K", C.c_int32), ("dtype", C.c_int32), ("weight_dtype", C.c_int32),
+                ("quant", C.c_int32), ("eps", C.c_float),
+                ("x", C.c_void_p), ("x_ld", C.c_int64), ("x_hd", C.c_int64), ("weight", C.c_void_p),
+                ("residual", C.c_void_p), ("residual_ld", C.c_int64), ("residual_hd", C.c_int64),
+                ("residual_out", C.c_void_p), ("residual_out_ld", C.c_int64), ("residual_out_hd", C.c_int64),
+                ("y", C.c_void_p), ("y_ld", C.c_int64), ("y_hd", C.c_int64), ("codes", C.c_void_p), ("scales", C.c_void_p)]
 
 
 # every symbol include/onebase_b200.h declares: name -> (restype, argtypes)
@@ -94,6 +104,9 @@ SYMBOLS = {
     "ob_nvfp4_packed_scale_bytes": (C.c_int, [C.c_int32, C.c_int32, C.POINTER(C.c_int32), C.POINTER(C.c_size_t)]),
     "ob_nvfp4_pack_scales": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.POINTER(C.c_int32), C.c_void_p, C.c_size_t,
                                        C.c_void_p]),
+    "ob_rms_norm": (C.c_int, [C.POINTER(ObRmsNorm), C.c_void_p]),
+    "ob_mxfp4_quantize": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "ob_mxfp4_dequantize": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p]),
     "ob_segment_index": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                    C.c_void_p, C.c_void_p]),
     "ob_comm_bytes": (C.c_int, [C.c_size_t, C.POINTER(C.c_size_t)]),

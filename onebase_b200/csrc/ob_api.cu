@@ -37,6 +37,10 @@ cudaError_t launch_k2_stream(const K2Params& p, const CUtensorMap& tm_w, const C
                              int grid, size_t smem, int fp4, int pdl, cudaStream_t stream);
 cudaError_t launch_pack_scales(const uint8_t* linear, int K, int S, const int32_t* widths, uint8_t* packed, size_t bytes,
                                cudaStream_t stream);
+cudaError_t launch_rms_norm(const ObRmsNorm& p, cudaStream_t stream);
+cudaError_t launch_mxfp4_quantize(const void* x, int dtype, long long rows, int K, long long ldx, void* codes, void* scales, cudaStream_t stream);
+cudaError_t launch_mxfp4_dequantize(const void* codes, const void* scales, int dtype, long long rows, int K, void* out, long long ldo,
+                                    cudaStream_t stream);
 cudaError_t launch_segment_index(const int32_t* token_lora, int M, int L, int32_t* tok, int32_t* srt, int32_t* seg_n,
                                  int32_t* seg_start, int32_t* seg_ids, cudaStream_t stream);
 struct ArParams {
@@ -1083,6 +1087,70 @@ int ob_requant_nvfp4(const void* src, int32_t l, int32_t rows, int32_t cols, voi
         return OB_ERR_ALIGN;
     cudaError_t e = launch_requant_nvfp4(src, l, rows, cols, packed, sf, inv_global, static_cast<unsigned int*>(amax_scratch),
                                          static_cast<cudaStream_t>(cuda_stream));
+    return e == cudaSuccess ? OB_OK : (int)e;
+}
+
+namespace {
+bool aligned_to(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// Strides of a [M, H, K] tensor whose rows are written: no two rows may share an element.
+bool rows_apart(int64_t ld, int64_t hd, int64_t M, int64_t H, int64_t K) {
+    if (ld < 0 || hd < 0) return false;
+    if (H == 1) return M == 1 || ld >= K;
+    if (M == 1) return hd >= K;
+    return (hd >= K && ld >= (H - 1) * hd + K) || (ld >= K && hd >= (M - 1) * ld + K);
+}
+}  // namespace
+
+int ob_rms_norm(const ObRmsNorm* n, void* cuda_stream) {
+    if (!n) return OB_ERR_NULL;
+    if (n->M < 0 || n->H < 1 || n->K < 1 || (int64_t)n->M * n->H > 0x7fffffffLL) return OB_ERR_SHAPE;
+    if (n->dtype != OB_DTYPE_BF16 && n->dtype != OB_DTYPE_F16) return OB_ERR_FORMAT;
+    if (n->weight && n->weight_dtype != n->dtype && n->weight_dtype != OB_DTYPE_F32) return OB_ERR_FORMAT;
+    if (n->quant != OB_QUANT_NONE && n->quant != OB_QUANT_FP8 && n->quant != OB_QUANT_MXFP4) return OB_ERR_FORMAT;
+    if (n->quant == OB_QUANT_MXFP4 && n->K % 32 != 0) return OB_ERR_SHAPE;
+    if (!(n->eps >= 0.0f)) return OB_ERR_SHAPE;
+    if (n->M == 0) return OB_OK;
+    if (!n->x || (n->quant != OB_QUANT_NONE && (!n->codes || !n->scales))) return OB_ERR_NULL;
+    if (!n->y && !n->residual_out && n->quant == OB_QUANT_NONE) return OB_ERR_NULL;      // nothing to give
+    if (n->x_ld < 0 || n->x_hd < 0 || (n->residual && (n->residual_ld < 0 || n->residual_hd < 0))) return OB_ERR_SHAPE;
+    if (n->y && !rows_apart(n->y_ld, n->y_hd, n->M, n->H, n->K)) return OB_ERR_SHAPE;
+    if (n->residual_out && !rows_apart(n->residual_out_ld, n->residual_out_hd, n->M, n->H, n->K)) return OB_ERR_SHAPE;
+    if (n->y && n->y == n->residual_out) return OB_ERR_SHAPE;
+    if (!aligned_to(n->x, 2) || !aligned_to(n->residual, 2) || !aligned_to(n->residual_out, 2) || !aligned_to(n->y, 2) ||
+        !aligned_to(n->weight, n->weight_dtype == OB_DTYPE_F32 ? 4 : 2))
+        return OB_ERR_ALIGN;
+    if ((n->quant == OB_QUANT_FP8 && (!aligned_to(n->codes, 8) || !aligned_to(n->scales, 4))) ||
+        (n->quant == OB_QUANT_MXFP4 && !aligned_to(n->codes, 4)))
+        return OB_ERR_ALIGN;
+    cudaError_t e = launch_rms_norm(*n, static_cast<cudaStream_t>(cuda_stream));
+    return e == cudaSuccess ? OB_OK : (int)e;
+}
+
+namespace {
+int mx_validate(const void* codes, const void* scales, int32_t dtype, int64_t rows, int32_t K, const void* dense, int64_t ld) {
+    if (dtype != OB_DTYPE_BF16 && dtype != OB_DTYPE_F16 && dtype != OB_DTYPE_F32) return OB_ERR_FORMAT;
+    if (rows < 0 || K < 32 || K % 32 != 0 || ld < 0 || rows > (INT64_MAX >> 8) / K) return OB_ERR_SHAPE;
+    if (rows == 0) return OB_OK;
+    if (!codes || !scales || !dense) return OB_ERR_NULL;
+    if (!aligned_to(codes, 4) || !aligned_to(dense, dtype == OB_DTYPE_F32 ? 4 : 2)) return OB_ERR_ALIGN;
+    return OB_OK;
+}
+}  // namespace
+
+int ob_mxfp4_quantize(const void* x, int32_t dtype, int64_t rows, int32_t K, int64_t ldx, void* codes, void* scales, void* cuda_stream) {
+    const int st = mx_validate(codes, scales, dtype, rows, K, x, ldx);
+    if (st != OB_OK || rows == 0) return st;
+    cudaError_t e = launch_mxfp4_quantize(x, dtype, rows, K, ldx, codes, scales, static_cast<cudaStream_t>(cuda_stream));
+    return e == cudaSuccess ? OB_OK : (int)e;
+}
+
+int ob_mxfp4_dequantize(const void* codes, const void* scales, int32_t dtype, int64_t rows, int32_t K, void* out, int64_t ldo,
+                        void* cuda_stream) {
+    const int st = mx_validate(codes, scales, dtype, rows, K, out, ldo);
+    if (st != OB_OK || rows == 0) return st;
+    if (rows > 1 && ldo < K) return OB_ERR_SHAPE;             // rows would overwrite one another
+    cudaError_t e = launch_mxfp4_dequantize(codes, scales, dtype, rows, K, out, ldo, static_cast<cudaStream_t>(cuda_stream));
     return e == cudaSuccess ? OB_OK : (int)e;
 }
 

@@ -1,0 +1,84 @@
+"""Root-mean-square norm with the residual's addition before it and low-precision codes behind it, on B200 through
+libonebase_b200.so (ob_rms_norm).
+
+In a decoder layer it stands in front of qkv_proj and gate_up_proj, and, on [tokens, heads, head size], it is the norm of queries and keys.  The reference leaves the norm to vLLM (RMSNorm,
+vllm/model_executor/layers/layernorm.py).
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple, Optional
+
+import torch
+
+from onebase_b200 import _lib
+
+_DTYPE = {torch.bfloat16: _lib.OB_DTYPE_BF16, torch.float16: _lib.OB_DTYPE_F16, torch.float32: _lib.OB_DTYPE_F32}
+_QUANT = {None: _lib.OB_QUANT_NONE, "fp8": _lib.OB_QUANT_FP8, "mxfp4": _lib.OB_QUANT_MXFP4}
+
+
+class NormOut(NamedTuple):
+    y: Optional[torch.Tensor]          # the norm, dtype of x (None under store=False)
+    residual: Optional[torch.Tensor]   # x + residual, dtype of x (None without a residual)
+    codes: Optional[torch.Tensor]      # "fp8": float8_e4m3fn, shape of x; "mxfp4": packed e2m1 uint8 [..., K/2]
+    scales: Optional[torch.Tensor]     # "fp8": fp32 [...]; "mxfp4": exponent + 127, uint8 [..., K/32]
+
+
+def _strides(t: torch.Tensor) -> tuple[int, int]:
+    return t.stride(0), (t.stride(1) if t.dim() == 3 else 0)
+
+
+def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 1e-6, *, residual: Optional[torch.Tensor] = None,
+             residual_out: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, store: bool = True,
+             quant: Optional[str] = None) -> NormOut:
+    """x [M, K] or [M, H, K] (bf16 or fp16, the last dimension dense, any other strides); weight [K] of x's dtype or fp32, or
+    None; residual of x's shape and dtype: s = x + residual is returned (in residual_out if given: it may be the residual
+    itself) and s is what is normed.  y = (s * weight) / sqrt(mean(s^2) + eps) goes to `out` (it may be x), or nowhere with
+    store=False.  quant = "fp8" or "mxfp4" also returns the codes of y before its rounding to 16 bits, with their scales."""
+    if x.device.type != "cuda":
+        raise RuntimeError("onebase_b200 runs on CUDA devices only (there is no CPU path)")
+    if x.dim() not in (2, 3) or x.dtype not in (torch.bfloat16, torch.float16) or x.shape[-1] < 1 or x.stride(-1) != 1 and x.shape[-1] > 1:
+        raise ValueError("rms_norm: x must be [M, K] or [M, H, K], bf16 or fp16, its last dimension dense")
+    if quant not in _QUANT:
+        raise ValueError("rms_norm: quant must be None, 'fp8' or 'mxfp4'")
+    K = x.shape[-1]
+    H = x.shape[1] if x.dim() == 3 else 1
+    if H < 1:
+        raise ValueError("rms_norm: x has no heads")
+    if weight is not None and (weight.shape != (K,) or weight.dtype not in (x.dtype, torch.float32) or weight.device != x.device or
+                               not weight.is_contiguous()):
+        raise ValueError("rms_norm: weight must be a dense [K] tensor on x's device, of x's dtype or fp32")
+    if residual_out is not None and residual is None:
+        raise ValueError("rms_norm: residual_out without a residual")
+    if out is not None and not store:
+        raise ValueError("rms_norm: out with store=False")
+    for name, t in (("residual", residual), ("residual_out", residual_out), ("out", out)):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.device != x.device or t.stride(-1) != 1 and K > 1):
+            raise ValueError(f"rms_norm: {name} must have x's shape, dtype and device, its last dimension dense")
+    y = None if not store else torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+    if residual is not None and residual_out is None:
+        residual_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    codes = scales = None
+    if quant == "fp8":
+        codes = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+        scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    elif quant == "mxfp4":
+        if K % 32:
+            raise ValueError("rms_norm: MXFP4 codes need K to be a multiple of 32")
+        codes = torch.empty(*x.shape[:-1], K // 2, dtype=torch.uint8, device=x.device)
+        scales = torch.empty(*x.shape[:-1], K // 32, dtype=torch.uint8, device=x.device)
+    n = _lib.ObRmsNorm()
+    n.M, n.H, n.K, n.dtype, n.quant, n.eps = x.shape[0], H, K, _DTYPE[x.dtype], _QUANT[quant], eps
+    n.x, (n.x_ld, n.x_hd) = x.data_ptr(), _strides(x)
+    if weight is not None:
+        n.weight, n.weight_dtype = weight.data_ptr(), _DTYPE[weight.dtype]
+    if residual is not None:
+        n.residual, (n.residual_ld, n.residual_hd) = residual.data_ptr(), _strides(residual)
+        n.residual_out, (n.residual_out_ld, n.residual_out_hd) = residual_out.data_ptr(), _strides(residual_out)
+    if y is not None:
+        n.y, (n.y_ld, n.y_hd) = y.data_ptr(), _strides(y)
+    if codes is not None:
+        n.codes, n.scales = codes.data_ptr(), scales.data_ptr()
+    with torch.cuda.device(x.device):
+        _lib.call("ob_rms_norm", C.byref(n), C.c_void_p(torch.cuda.current_stream(x.device).cuda_stream))
+    return NormOut(y, residual_out, codes, scales)

@@ -50,8 +50,8 @@ extern "C" {
                                     can: the tensor-core shrink's launch did not cover them; word 2 = work items found,
                                     word 3 = work items launched */
 
-enum { OB_BASE_FP8 = 0, OB_BASE_NVFP4 = 1 };
-enum { OB_X_PLAIN = 0, OB_X_SILU_MUL = 1 };
+enum { OB_BASE_FP8 = 0, OB_BASE_NVFP4 = 1, OB_BASE_MXFP4 = 2 };
+enum { OB_X_PLAIN = 0, OB_X_SILU_MUL = 1, OB_X_QUANTIZED = 2 };
 enum { OB_LORA_BF16 = 0, OB_LORA_FP8 = 1, OB_LORA_NVFP4 = 2 };
 
 #define OB_MAX_SLICES 4
@@ -72,12 +72,13 @@ typedef struct ObLayerDesc {
     int32_t R;                       /* LoRA rank: 16, 32, 64, 128 or 256 */
     int32_t widths[OB_MAX_SLICES];   /* N_s, sum = N */
     int32_t max_m;                   /* largest token count of a call */
-    const void* w_q;                 /* FP8: [N,K] e4m3.  NVFP4: [N,K/2] packed e2m1, element 2i in the low nibble */
+    const void* w_q;                 /* FP8: [N,K] e4m3.  NVFP4, MXFP4: [N,K/2] packed e2m1, element 2i in the low nibble */
     const void* w_sf;                /* NVFP4: ue4m3 block scales PACKED by ob_nvfp4_pack_scales from the checkpoint's linear
-                                        [N,K/16] layout (ob_nvfp4_packed_scale_bytes bytes).  FP8: null */
+                                        [N,K/16] layout (ob_nvfp4_packed_scale_bytes bytes).  MXFP4: exponent + 127 bytes packed by
+                                        ob_mxfp4_pack_scales from [N,K/32].  FP8: null */
     const float* s_w;                /* FP8: [1] per-tensor weight scale */
     const float* x_global;           /* NVFP4: [1] static activation global scale (1 / input_scale) */
-    const float* alpha;              /* NVFP4: [1] 1 / (x_global * w_global) */
+    const float* alpha;              /* NVFP4: [1] 1 / (x_global * w_global).  MXFP4: [1] factor of the base product (1: none) */
     const void* a[OB_MAX_SLICES];    /* adapter A per slice: bf16 [L,1,R,K] | e4m3 [L,1,R,K] | packed [L,1,R,K/2] */
     const void* b[OB_MAX_SLICES];    /* adapter B per slice: bf16 [L,1,N_s,R] | e4m3 | packed [L,1,N_s,R/2] */
     const void* sa[OB_MAX_SLICES];   /* FP8: fp32 [L,R] row scales.  NVFP4: ue4m3 [L,1,R,K/16] block scales */
@@ -120,6 +121,12 @@ typedef struct ObBatch {
     int32_t x_op;
     const void* residual;
     int64_t ldr;
+    /*   x_op = OB_X_QUANTIZED   x has been quantized already (ob_rms_norm, ob_mxfp4_quantize): K1 takes these codes into its
+     *        order instead of making its own, and x itself -- still [M, K] bf16 -- is what the adapters multiply.  FP8 base:
+     *        x_codes [M, K] e4m3, x_scales [M] fp32; MXFP4 base: x_codes [M, K/2], x_scales [M, K/32]; dense, x_codes 16-byte aligned.
+     *        The NVFP4 base refuses it.  Not read under the other values of x_op. */
+    const void* x_codes;
+    const void* x_scales;
 } ObBatch;
 
 /* Capacity of a shared workspace (what the reference's Scratch.ensure / _Work.ensure grow,
@@ -253,6 +260,21 @@ int ob_k2_nvfp4(ObLayer* layer, const ObBatch* batch, void* workspace, const ObW
 int ob_chain_nvfp4(ObLayer* layer, const ObBatch* batch, void* workspace, const ObWorkspaceShape* shape,
                    const ObTileCfg* cfg, void* cuda_stream);
 
+/* The MXFP4-base counterparts: K1 quantizes x to e2m1 codes with a power-of-two scale per 32 elements (ob_mxfp4_quantize's rule) and
+ * shrinks; K2 is the block-scaled tcgen05 GEMM (kind::mxf4), y = alpha sum v(x) v(w) + LoRA, K a multiple of 32 (the large prefill tiles: of
+ * 256).  The persistent and the one-kernel decode forms (ObTileCfg.stream, .fused) do not exist for this base: asked for, the call takes
+ * the two-kernel chain.  No counterpart in the reference (its 4-bit base is NVFP4). */
+int ob_k1_mxfp4(ObLayer* layer, const ObBatch* batch, void* workspace, const ObWorkspaceShape* shape, const ObTileCfg* cfg, void* cuda_stream);
+int ob_k2_mxfp4(ObLayer* layer, const ObBatch* batch, void* workspace, const ObWorkspaceShape* shape, const ObTileCfg* cfg, int pdl,
+                void* cuda_stream);
+int ob_chain_mxfp4(ObLayer* layer, const ObBatch* batch, void* workspace, const ObWorkspaceShape* shape, const ObTileCfg* cfg,
+                   void* cuda_stream);
+/* One-time re-layout of an MXFP4 weight's scale bytes from linear [N, K/32] into the order K2 copies to TMEM: per (128-row output tile
+ * of a slice, 256-element K slot) two 512-byte atoms [row % 32][row / 32][4 scales], zero padded. */
+int ob_mxfp4_packed_scale_bytes(int32_t K, int32_t S, const int32_t* widths, size_t* bytes);
+int ob_mxfp4_pack_scales(const void* w_sf_linear, int32_t K, int32_t S, const int32_t* widths, void* packed, size_t packed_bytes,
+                         void* cuda_stream);
+
 /* One-time re-layout of an NVFP4 weight's block scales from the checkpoint's linear [N, K/16] ue4m3 matrix (what the
  * reference keeps before vLLM swizzles it, lowbit_lora/plugin.py:155-174) into the order K2 copies to TMEM: per
  * (128-row output tile of a slice, 256-element K slot) four 512-byte atoms [row % 32][row / 32][4 scales], zero padded.
@@ -279,7 +301,8 @@ int ob_requant_nvfp4(const void* src, int32_t l, int32_t rows, int32_t cols, voi
  *     OB_QUANT_FP8     codes [M * H, K] e4m3 with scales [M * H] fp32 = max(max|y| / 448, 1 / (448 * 512)): the layout and the
  *                      scale's floor of ob_k1_fp8's own quantization
  *     OB_QUANT_MXFP4   codes [M * H, K/2] and scales [M * H, K/32] as ob_mxfp4_quantize gives them
- * Strides are in elements: `*_ld` between tokens, `*_hd` between a token's heads (H = 1: unused).  An output may be the same memory as an input of the same strides, else they must not
+ * which ob_chain_fp8 / ob_chain_mxfp4 take as ObBatch.x_codes / x_scales.  Strides are in elements: `*_ld` between tokens, `*_hd`
+ * between a token's heads (H = 1: unused).  An output may be the same memory as an input of the same strides, else they must not
  * overlap.  A row that holds a NaN or an infinity has NaN for its scale and codes (and for its y, but for zeros where an infinity divides a
  * number).  One launch, capturable, no workspace; M = 0 does nothing.  No counterpart in the reference, which leaves the norm to
  * vLLM (RMSNorm, vllm/model_executor/layers/layernorm.py). */

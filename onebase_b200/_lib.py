@@ -14,9 +14,9 @@ LIB_PATH = PKG / "lib" / "libonebase_b200.so"
 
 OB_MAX_SLICES = 4
 OB_STATUS_WORDS = 16
-OB_BASE_FP8, OB_BASE_NVFP4 = 0, 1
+OB_BASE_FP8, OB_BASE_NVFP4, OB_BASE_MXFP4 = 0, 1, 2
 OB_LORA_BF16, OB_LORA_FP8, OB_LORA_NVFP4 = 0, 1, 2
-OB_X_PLAIN, OB_X_SILU_MUL = 0, 1
+OB_X_PLAIN, OB_X_SILU_MUL, OB_X_QUANTIZED = 0, 1, 2
 OB_WS = {name: i for i, name in enumerate(("status", "counters", "sx", "xq", "xsf", "hp", "part", "xs", "hb", "hcat"))}
 
 
@@ -42,6 +42,7 @@ class ObBatch(C.Structure):
         ("M", C.c_int32), ("x", C.c_void_p), ("ldx", C.c_int64), ("y", C.c_void_p), ("ldy", C.c_int64),
         ("tok", C.c_void_p), ("srt", C.c_void_p), ("seg_n", C.c_void_p), ("seg_start", C.c_void_p), ("seg_ids", C.c_void_p),
         ("x_op", C.c_int32), ("residual", C.c_void_p), ("ldr", C.c_int64),
+        ("x_codes", C.c_void_p), ("x_scales", C.c_void_p),
     ]
 
 
@@ -101,6 +102,15 @@ SYMBOLS = {
                               C.c_int, C.c_void_p]),
     "ob_chain_nvfp4": (C.c_int, [C.c_void_p, C.POINTER(ObBatch), C.c_void_p, C.POINTER(ObWorkspaceShape),
                                  C.POINTER(ObTileCfg), C.c_void_p]),
+    "ob_k1_mxfp4": (C.c_int, [C.c_void_p, C.POINTER(ObBatch), C.c_void_p, C.POINTER(ObWorkspaceShape), C.POINTER(ObTileCfg),
+                              C.c_void_p]),
+    "ob_k2_mxfp4": (C.c_int, [C.c_void_p, C.POINTER(ObBatch), C.c_void_p, C.POINTER(ObWorkspaceShape), C.POINTER(ObTileCfg),
+                              C.c_int, C.c_void_p]),
+    "ob_chain_mxfp4": (C.c_int, [C.c_void_p, C.POINTER(ObBatch), C.c_void_p, C.POINTER(ObWorkspaceShape),
+                                 C.POINTER(ObTileCfg), C.c_void_p]),
+    "ob_mxfp4_packed_scale_bytes": (C.c_int, [C.c_int32, C.c_int32, C.POINTER(C.c_int32), C.POINTER(C.c_size_t)]),
+    "ob_mxfp4_pack_scales": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.POINTER(C.c_int32), C.c_void_p, C.c_size_t,
+                                       C.c_void_p]),
     "ob_nvfp4_packed_scale_bytes": (C.c_int, [C.c_int32, C.c_int32, C.POINTER(C.c_int32), C.POINTER(C.c_size_t)]),
     "ob_nvfp4_pack_scales": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.POINTER(C.c_int32), C.c_void_p, C.c_size_t,
                                        C.c_void_p]),

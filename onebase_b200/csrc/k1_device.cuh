@@ -1,6 +1,7 @@
 // Device code of K1 -- activation quantization of one tile position and the LoRA shrink of one warp's unit -- shared by
 // the stand-alone K1 kernel and by the fused decode kernel, whose warps run the same units before their GEMM roles.
 #pragma once
+#include "mxfp4.cuh"
 #include "ob_common.cuh"
 #include "ob_ptx.cuh"
 
@@ -43,10 +44,10 @@ __device__ __forceinline__ uint2 quant8(const uint4& v, float sx) {
 // it: silu in fp32, rounded to bf16, times up, rounded to bf16 (activation.py, forward_native).
 // XOP is a template parameter: the plain kernels must not carry the activation's code (after an L2 flush every
 // instruction line of a launch is a cold fetch, and K1 sits on the chain's critical path).
-template <bool XOP>
+template <int XOP>
 __device__ __forceinline__ uint4 x_load8(const K1Params& p, const __nv_bfloat16* xrow, int k) {
     const uint4 g = __ldg(reinterpret_cast<const uint4*>(xrow + k));
-    if (!XOP) return g;
+    if (XOP != OB_X_SILU_MUL) return g;
     const uint4 u = __ldg(reinterpret_cast<const uint4*>(xrow + p.K + k));
     const uint32_t gw[4] = {g.x, g.y, g.z, g.w}, uw[4] = {u.x, u.y, u.z, u.w};
     uint32_t o[4];
@@ -73,7 +74,7 @@ __device__ __forceinline__ int row_of_position(const K1Params& p, int pos, int l
 // NT threads (tid in [0, NT)) that meet at named barrier BAR quantize row `row` of x into position `pos`.
 // COPY: pass 1 also leaves the row's bf16 values in the adapter-sorted copy p.xs, and pass 2 takes them from there (every
 // thread what it wrote itself) instead of forming them again.
-template <int NT, int BAR, bool XOP = false, bool COPY = false>
+template <int NT, int BAR, int XOP = OB_X_PLAIN, bool COPY = false>
 __device__ void quantize_row(const K1Params& p, int pos, int row, int tid) {
     __shared__ float s_part[NT / 32];
     __shared__ float s_scale;
@@ -115,7 +116,7 @@ __device__ void quantize_row(const K1Params& p, int pos, int row, int tid) {
 // registers: thousands of such CTAs keep the code warm, so the unrolled second pass costs no cold fetches, and a row
 // of up to 4096 elements needs so few registers that eight CTAs share an SM.  With the input transform it is formed once
 // (the rolled form evaluates it in both passes and a third time for the copy).
-template <int NT, int BAR, int NV, bool XOP = false>
+template <int NT, int BAR, int NV, int XOP = OB_X_PLAIN>
 __device__ void quantize_row_regs(const K1Params& p, int pos, int row, int tid) {
     __shared__ float s_part[NT / 32];
     __shared__ float s_scale;
@@ -187,7 +188,7 @@ __device__ __forceinline__ float e4m3_to_float(uint32_t code) {
 // [r/32][4], r = position within the token tile.
 // COPY: also write the row's bf16 values to the adapter-sorted copy p.xs (prefill: the tensor-core shrink's input) from
 // the vectors just loaded, instead of a second pass over the row.
-template <int NT, bool XOP = false, bool COPY = false>
+template <int NT, int XOP = OB_X_PLAIN, bool COPY = false>
 __device__ void quantize_row_nvfp4(const K1Params& p, int pos, int row, int tid) {
     const float gs = __ldg(p.x_global);
     const __nv_bfloat16* xr = p.x + (int64_t)row * p.ldx;
@@ -240,6 +241,58 @@ __device__ void quantize_row_nvfp4(const K1Params& p, int pos, int row, int tid)
         }
         // K slot b / 16, MMA (b % 16) / 4, scale b % 4; blocks past K are zero scales
         sf_tile[(size_t)(b >> 4) * p.nblk * kSfSlotBytes + sf_row + ((b & 15) >> 2) * 512 + (b & 3)] = (uint8_t)sf_code;
+    }
+}
+
+// Where the scale byte of 32-element block `b` of position `pos` lies in K2's scale-factor atoms (MXFP4): [token tile][K slot]
+// [128-token block][pair of MMAs][r%32][r/32][4], r = position within the token tile.
+__device__ __forceinline__ uint8_t* mx_scale_slot(const K1Params& p, int pos, int b) {
+    constexpr int kSlot = sf_slot_bytes(OB_BASE_MXFP4);
+    const int mt = pos / p.tn, r = pos % p.tn;
+    return p.xsf + (((size_t)mt * p.kslots + (size_t)(b >> 3)) * p.nblk + (size_t)(r >> 7)) * kSlot + ((b >> 2) & 1) * 512 + (r & 31) * 16 +
+           ((r & 127) >> 5) * 4 + (b & 3);
+}
+
+// MXFP4 activation quantization of one position (the rule of mxfp4.cuh): four lanes per block of 32, eight elements each, so a
+// warp's loads and stores are dense.  Blocks past K in the last K slot get scale byte 0 (their codes are zeros by TMA's fill).
+template <int NT, int XOP = OB_X_PLAIN, bool COPY = false>
+__device__ void quantize_row_mxfp4(const K1Params& p, int pos, int row, int tid) {
+    const __nv_bfloat16* xr = p.x + (int64_t)row * p.ldx;
+    const int groups = p.K >> 3;
+    uint32_t* out = reinterpret_cast<uint32_t*>(p.xq + (size_t)pos * (size_t)(p.K >> 1));
+#pragma unroll 2
+    for (int i = tid; i < p.kslots * 32; i += NT) {   // (whole warps: a K slot has 32 groups of eight)
+        const uint4 u = i < groups ? x_load8<XOP>(p, xr, i * 8) : make_uint4(0u, 0u, 0u, 0u);
+        if (COPY && p.xs != nullptr && i < groups) reinterpret_cast<uint4*>(p.xs + (size_t)pos * (size_t)p.K)[i] = u;
+        float v[8];
+        unpack8(u, v);
+        uint32_t byte;
+        const uint32_t codes = mx_quantize8(v, byte);
+        if (i < groups) out[i] = codes;
+        if ((i & 3) == 0) *mx_scale_slot(p, pos, i >> 2) = (uint8_t)byte;
+    }
+}
+
+// OB_X_QUANTIZED: row `row` of the caller's codes and scales to position `pos` (COPY: and the row of x to the sorted copy).
+template <int NT, int BASE, bool COPY = false>
+__device__ void take_row_codes(const K1Params& p, int pos, int row, int tid) {
+    const int row_bytes = BASE == OB_BASE_FP8 ? p.K : p.K >> 1;   // (a multiple of 16)
+    const uint4* src = reinterpret_cast<const uint4*>(p.x_codes + (size_t)row * (size_t)row_bytes);
+    uint4* dst = reinterpret_cast<uint4*>(p.xq + (size_t)pos * (size_t)row_bytes);
+#pragma unroll 2
+    for (int i = tid; i < (row_bytes >> 4); i += NT) dst[i] = src[i];
+    if (BASE == OB_BASE_FP8) {
+        if (tid == 0) p.sx[pos] = reinterpret_cast<const float*>(p.x_scales)[row];
+    } else {
+        const int blocks = p.K >> 5;
+        const uint8_t* sc = p.x_scales + (size_t)row * (size_t)blocks;
+        for (int b = tid; b < p.kslots * 8; b += NT) *mx_scale_slot(p, pos, b) = b < blocks ? sc[b] : (uint8_t)0;
+    }
+    if (COPY && p.xs != nullptr) {
+        const uint4* xr = reinterpret_cast<const uint4*>(p.x + (int64_t)row * p.ldx);
+        uint4* xo = reinterpret_cast<uint4*>(p.xs + (size_t)pos * (size_t)p.K);
+#pragma unroll 2
+        for (int i = tid; i < (p.K >> 3); i += NT) xo[i] = xr[i];
     }
 }
 
@@ -339,7 +392,7 @@ __device__ __forceinline__ float post_scale(const K1Params& p, int lora, int s, 
 // One pass of a warp: 8 rank rows [k0, k1) of adapter `lora`, slice s, times the `nt` (<= 4) tokens whose x rows are
 // rows[0..nt); writes the split-K partial hp[j][s][pos0 + t][rg*8 .. +8].  bf16 adapters.  The first block of A is
 // requested before the wait on the preceding kernel (A is static); x is read and hp written only after it.
-template <int FMT, bool XOP = false>
+template <int FMT, int XOP = OB_X_PLAIN>
 __device__ __forceinline__ void shrink_pass(const K1Params& p, int lora, int s, int rg, int j, int k0, int k1, int pos0,
                                                  const int* rows, int nt, int lane) {
     const ARows<FMT> a(p, lora, s, rg);
@@ -401,7 +454,7 @@ __device__ __forceinline__ void fma8(float (&acc)[8], const uint4 (&av)[8], cons
 
 // Decode form of the pass (one token): two K steps of A in flight per lane (8 KB per warp), both requested before the wait
 // on the preceding kernel.  8 lane-partials -> lanes 0..7 hold the 8 rank rows' sums (2 butterfly + 3 transposing steps).
-template <int FMT, bool XOP = false>
+template <int FMT, int XOP = OB_X_PLAIN>
 __device__ __forceinline__ void shrink_pass1(const K1Params& p, int lora, int s, int rg, int j, int k0, int k1, int pos,
                                                   int row, int lane) {
     const ARows<FMT> a(p, lora, s, rg);
@@ -452,7 +505,7 @@ __device__ __forceinline__ void shrink_pass1(const K1Params& p, int lora, int s,
 // One warp-wide read of the segment index gives the batch totals and the segment (adapter) of each of the warp's
 // positions; the positions' token rows are requested at the same time.  Then one pass per run of positions that share
 // an adapter.
-template <int FMT, bool XOP = false>
+template <int FMT, int XOP = OB_X_PLAIN>
 __device__ void shrink_unit(const K1Params& p, int pb, int u, int lane) {
     const int p0 = pb * p.pb;
     int rows[4];

@@ -1,5 +1,6 @@
-// K1: activation quantization -- per-token dynamic e4m3 for an FP8 base, or e2m1 codes with one ue4m3 scale per 16
-// elements against a static global scale for an NVFP4 base -- fused in one launch with every tenant's LoRA shrink
+// K1: activation quantization -- per-token dynamic e4m3 for an FP8 base, e2m1 codes with one ue4m3 scale per 16
+// elements against a static global scale for an NVFP4 base, or with one power-of-two scale per 32 for an MXFP4 base; or codes that
+// the caller brings -- fused in one launch with every tenant's LoRA shrink
 // h = x A^T.
 //
 // One launch, two kinds of CTA (256 threads each):
@@ -25,19 +26,27 @@ namespace ob {
 
 constexpr int kK1Threads = 256;
 
+template <int NT, int BASE, int XOP, bool COPY = false>
+__device__ __forceinline__ void position_codes(const K1Params& p, int pos, int row, int tid) {
+    if constexpr (XOP == OB_X_QUANTIZED) take_row_codes<NT, BASE, COPY>(p, pos, row, tid);
+    else if constexpr (BASE == OB_BASE_MXFP4) quantize_row_mxfp4<NT, XOP, COPY>(p, pos, row, tid);
+    else if constexpr (BASE == OB_BASE_NVFP4) quantize_row_nvfp4<NT, XOP, COPY>(p, pos, row, tid);
+    else quantize_row<NT, 0, XOP, COPY>(p, pos, row, tid);
+}
+
 // One instantiation per (adapter storage, base format): each launch carries only the code of its own case.
 // LOOPED: the one-CTA-per-SM form that runs beside the persistent GEMM; a function of its own, because the shared-memory
 // carve-out it needs (see launch_k1_impl) is a per-function attribute and costs the other form its L1 cache.
-// XOP: the projection's input is formed from x on the fly (OB_X_SILU_MUL); plain launches run an instantiation without it.
-template <int LORA_FMT, bool FP4_BASE, bool LOOPED, bool XOP>
-__global__ void __launch_bounds__(kK1Threads, XOP ? 2 : 0) k1_kernel(const K1Params p) {
+// XOP: the projection's input is formed from x on the fly (OB_X_SILU_MUL), or its codes are given (OB_X_QUANTIZED); plain launches run
+// an instantiation without either.
+template <int LORA_FMT, int BASE, bool LOOPED, int XOP>
+__global__ void __launch_bounds__(kK1Threads, XOP == OB_X_SILU_MUL ? 2 : 0) k1_kernel(const K1Params p) {
     griddep_launch_dependents();
     OB_TRACE1(0)
     if ((int)blockIdx.x < p.n_quant_ctas) {
         const int row = row_of_position(p, blockIdx.x, threadIdx.x & 31);
         griddep_wait();                               // x comes from the preceding kernel; the scratch may still be read by it
-        if (FP4_BASE) quantize_row_nvfp4<kK1Threads, XOP>(p, blockIdx.x, row, threadIdx.x);
-        else quantize_row<kK1Threads, 0, XOP>(p, blockIdx.x, row, threadIdx.x);
+        position_codes<kK1Threads, BASE, XOP>(p, blockIdx.x, row, threadIdx.x);
         if (p.xs != nullptr) {                        // the tensor-core shrink reads x in position order by TMA
             const __nv_bfloat16* xr = p.x + (int64_t)row * p.ldx;
             uint4* xo = reinterpret_cast<uint4*>(p.xs + (size_t)blockIdx.x * (size_t)p.K);
@@ -71,19 +80,18 @@ __global__ void __launch_bounds__(kK1Threads, XOP ? 2 : 0) k1_kernel(const K1Par
 
 // Quantization alone, for batches whose shrink runs on the tensor cores: without the shrink's registers four of these
 // CTAs share an SM instead of two, which is what a launch of thousands of one-row CTAs needs.
-template <bool FP4_BASE, bool XOP>
+template <int BASE, int XOP>
 __global__ void __launch_bounds__(kK1Threads, 4) k1_quant_kernel(const K1Params p) {
     griddep_launch_dependents();
     const int row = row_of_position(p, blockIdx.x, threadIdx.x & 31);
     griddep_wait();
-    if (FP4_BASE) quantize_row_nvfp4<kK1Threads, XOP, true>(p, blockIdx.x, row, threadIdx.x);
-    else quantize_row<kK1Threads, 0, XOP, true>(p, blockIdx.x, row, threadIdx.x);
+    position_codes<kK1Threads, BASE, XOP, true>(p, blockIdx.x, row, threadIdx.x);
 }
 
 // The FP8 base's form of it with the row in registers (NV vectors per thread of NT threads): one read of x serves the amax, the
 // codes and the sorted copy.  MIN_CTAS per SM bounds the registers: the launch is bound by how many rows an SM has in flight
 // and, with the input transform, by its instructions.
-template <int NT, int NV, bool XOP, int MIN_CTAS>
+template <int NT, int NV, int XOP, int MIN_CTAS>
 __global__ void __launch_bounds__(NT, MIN_CTAS) k1_quant_regs_kernel(const K1Params p) {
     griddep_launch_dependents();
     const int row = row_of_position(p, blockIdx.x, threadIdx.x & 31);
@@ -107,22 +115,22 @@ static cudaError_t launch_quant_kernel(cudaLaunchConfig_t cfg, const K1Params& p
     return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
-template <bool FP4_BASE, bool XOP>
+template <int BASE, int XOP>
 static cudaError_t launch_quant_only(const cudaLaunchConfig_t& cfg, const K1Params& p) {
     static std::atomic<unsigned long long> carved{0};
-    if constexpr (!FP4_BASE) {
-        if (p.K <= 8 * 2 * 256) return launch_quant_kernel<256>(cfg, p, k1_quant_regs_kernel<256, 2, XOP, XOP ? 4 : 8>, &carved);
+    if constexpr (BASE == OB_BASE_FP8 && XOP != OB_X_QUANTIZED) {
+        if (p.K <= 8 * 2 * 256) return launch_quant_kernel<256>(cfg, p, k1_quant_regs_kernel<256, 2, XOP, XOP == OB_X_SILU_MUL ? 4 : 8>, &carved);
         // (with the transform 512 threads measured 4 us less at 200 rows of 12288, 2 us at 2048; without it they are equal)
-        if constexpr (XOP) {
-            if (p.K <= 8 * 3 * 512) return launch_quant_kernel<512>(cfg, p, k1_quant_regs_kernel<512, 3, true, 2>, nullptr);
+        if constexpr (XOP == OB_X_SILU_MUL) {
+            if (p.K <= 8 * 3 * 512) return launch_quant_kernel<512>(cfg, p, k1_quant_regs_kernel<512, 3, OB_X_SILU_MUL, 2>, nullptr);
         } else {
-            if (p.K <= 8 * 6 * 256) return launch_quant_kernel<256>(cfg, p, k1_quant_regs_kernel<256, 6, false, 4>, nullptr);
+            if (p.K <= 8 * 6 * 256) return launch_quant_kernel<256>(cfg, p, k1_quant_regs_kernel<256, 6, OB_X_PLAIN, 4>, nullptr);
         }
     }
-    return launch_quant_kernel<kK1Threads>(cfg, p, k1_quant_kernel<FP4_BASE, XOP>, nullptr);
+    return launch_quant_kernel<kK1Threads>(cfg, p, k1_quant_kernel<BASE, XOP>, nullptr);
 }
 
-template <int LORA_FMT, bool FP4_BASE>
+template <int LORA_FMT, int BASE>
 static cudaError_t launch_k1_impl(const K1Params& p, int grid, int pdl, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
@@ -134,38 +142,49 @@ static cudaError_t launch_k1_impl(const K1Params& p, int grid, int pdl, cudaStre
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl ? 1 : 0;
-    if (p.looped) {
-        // Beside the persistent GEMM, K1 needs next to no shared memory but must leave the SMs it runs on configured for the
-        // LARGEST shared-memory carve-out: the split between L1 and shared memory only changes on an idle SM, so with the
-        // default (small) carve-out the dependent GEMM's CTAs (150-200 KB each) could not become resident beside K1's and
-        // the two kernels of the chain would run one after the other.  (It costs this form most of its L1 cache.)
-        static std::atomic<unsigned long long> carved{0};
-        int dev = 0;
-        if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 && !(carved.load() & (1ull << dev))) {
-            cudaError_t e = cudaFuncSetAttribute(k1_kernel<LORA_FMT, FP4_BASE, true, false>, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                                 (int)cudaSharedmemCarveoutMaxShared);
-            if (e != cudaSuccess) return e;
-            carved.fetch_or(1ull << dev);
+    if constexpr (BASE != OB_BASE_MXFP4) {
+        if (p.looped) {
+            // Beside the persistent GEMM, K1 needs next to no shared memory but must leave the SMs it runs on configured for the
+            // LARGEST shared-memory carve-out: the split between L1 and shared memory only changes on an idle SM, so with the
+            // default (small) carve-out the dependent GEMM's CTAs (150-200 KB each) could not become resident beside K1's and
+            // the two kernels of the chain would run one after the other.  (It costs this form most of its L1 cache.)
+            static std::atomic<unsigned long long> carved{0};
+            int dev = 0;
+            if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 && !(carved.load() & (1ull << dev))) {
+                cudaError_t e = cudaFuncSetAttribute(k1_kernel<LORA_FMT, BASE, true, OB_X_PLAIN>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                                     (int)cudaSharedmemCarveoutMaxShared);
+                if (e != cudaSuccess) return e;
+                carved.fetch_or(1ull << dev);
+            }
+            return cudaLaunchKernelEx(&cfg, k1_kernel<LORA_FMT, BASE, true, OB_X_PLAIN>, p);
         }
-        return cudaLaunchKernelEx(&cfg, k1_kernel<LORA_FMT, FP4_BASE, true, false>, p);
     }
     // no shrink warps in this launch (the tensor-core shrink follows: the sorted copy of x is wanted).  SiLU * mul at 2048
     // rows of 12288: 127 us in k1_kernel<XOP> (two CTAs per SM, the transform evaluated three times)
-    if (grid == p.n_quant_ctas && p.xs != nullptr && p.xq_ready == nullptr && p.trace == nullptr)
-        return p.x_op != OB_X_PLAIN ? launch_quant_only<FP4_BASE, true>(cfg, p) : launch_quant_only<FP4_BASE, false>(cfg, p);
-    if (p.x_op != OB_X_PLAIN) return cudaLaunchKernelEx(&cfg, k1_kernel<LORA_FMT, FP4_BASE, false, true>, p);
-    return cudaLaunchKernelEx(&cfg, k1_kernel<LORA_FMT, FP4_BASE, false, false>, p);
+    const bool quant_only = grid == p.n_quant_ctas && p.xs != nullptr && p.xq_ready == nullptr && p.trace == nullptr;
+    if constexpr (BASE != OB_BASE_NVFP4) {
+        if (p.x_op == OB_X_QUANTIZED)
+            return quant_only ? launch_quant_only<BASE, OB_X_QUANTIZED>(cfg, p)
+                              : cudaLaunchKernelEx(&cfg, k1_kernel<LORA_FMT, BASE, false, OB_X_QUANTIZED>, p);
+    }
+    if (quant_only)
+        return p.x_op != OB_X_PLAIN ? launch_quant_only<BASE, OB_X_SILU_MUL>(cfg, p) : launch_quant_only<BASE, OB_X_PLAIN>(cfg, p);
+    if (p.x_op != OB_X_PLAIN) return cudaLaunchKernelEx(&cfg, k1_kernel<LORA_FMT, BASE, false, OB_X_SILU_MUL>, p);
+    return cudaLaunchKernelEx(&cfg, k1_kernel<LORA_FMT, BASE, false, OB_X_PLAIN>, p);
+}
+
+template <int LORA_FMT>
+static cudaError_t launch_k1_base(const K1Params& p, int grid, int pdl, cudaStream_t stream) {
+    return p.base_fmt == OB_BASE_NVFP4   ? launch_k1_impl<LORA_FMT, OB_BASE_NVFP4>(p, grid, pdl, stream)
+           : p.base_fmt == OB_BASE_MXFP4 ? launch_k1_impl<LORA_FMT, OB_BASE_MXFP4>(p, grid, pdl, stream)
+                                         : launch_k1_impl<LORA_FMT, OB_BASE_FP8>(p, grid, pdl, stream);
 }
 
 cudaError_t launch_k1_fp8(const K1Params& p, int grid, int pdl, cudaStream_t stream) {
-    const bool fp4 = p.base_fmt == OB_BASE_NVFP4;
     switch (p.lora_fmt) {
-        case kLoraFp8:
-            return fp4 ? launch_k1_impl<kLoraFp8, true>(p, grid, pdl, stream) : launch_k1_impl<kLoraFp8, false>(p, grid, pdl, stream);
-        case kLoraNvfp4:
-            return fp4 ? launch_k1_impl<kLoraNvfp4, true>(p, grid, pdl, stream) : launch_k1_impl<kLoraNvfp4, false>(p, grid, pdl, stream);
-        default:
-            return fp4 ? launch_k1_impl<kLoraBf16, true>(p, grid, pdl, stream) : launch_k1_impl<kLoraBf16, false>(p, grid, pdl, stream);
+        case kLoraFp8: return launch_k1_base<kLoraFp8>(p, grid, pdl, stream);
+        case kLoraNvfp4: return launch_k1_base<kLoraNvfp4>(p, grid, pdl, stream);
+        default: return launch_k1_base<kLoraBf16>(p, grid, pdl, stream);
     }
 }
 

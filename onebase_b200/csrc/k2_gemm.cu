@@ -1,5 +1,5 @@
 // K2: y = bf16( scale * (x_q W_q^T) + sum over tenants of h B^T ) for an FP8 (e4m3, scale = s_x * s_w) or NVFP4 (e2m1 with
-// ue4m3 block scales, scale = alpha) base, one CTA per (128 output features,
+// ue4m3 block scales, scale = alpha) or MXFP4 (e2m1 with power-of-two block scales) base, one CTA per (128 output features,
 // token tile, K split), two CTAs per SM, hand-written for sm_100a:
 //
 //   swap-AB orientation -- the 128 rows of the W tile sit on the MMA's M side, the tokens (16..256 per tile, adapter-
@@ -13,12 +13,13 @@
 //            x_q tiles are requested after griddepcontrol.wait.
 //   warp 1   allocates TMEM and issues tcgen05.mma: kind::f8f6f4 (e4m3 x e4m3, fp32) into accumulator 0 for the base
 //            GEMM -- or, for an NVFP4 base, kind::mxf4nvf4.block_scale.scale_vec::4X with both operands' ue4m3 block
-//            scales copied from the slot into TMEM by tcgen05.cp (warp 3) -- and kind::f16 (bf16) into accumulator 1 for each
+//            scales copied from the slot into TMEM by tcgen05.cp (warp 3); for an MXFP4 base kind::mxf4 with
+//            scale_vec::2X, whose scale atoms serve two MMAs each -- and kind::f16 (bf16) into accumulator 1 for each
 //            expand step; tcgen05.commit releases ring slots.  With stored adapters (FP8 / NVFP4 codes) a decode tile's B tiles
 //            are not in the ring: warps 4-7 convert them into tensor memory, where they are the MMA's A operand.
 //   warp 2   (decode tiles, <= 32 tokens) keeps masked H tiles ready: H of a step = the h rows of that tenant's tokens,
 //            zero elsewhere, in the UMMA layout; it only rewrites the one or two rows that change between steps.
-//   warp 3   NVFP4 base: copies each W slot's block scales to TMEM ahead of its MMAs.
+//   warp 3   NVFP4, MXFP4 base: copies each W slot's block scales to TMEM ahead of its MMAs.
 //   warps 4-7  read vLLM's segment index, list the (segment, rank chunk) expand steps of this tile; after K1 they sum
 //            its split-K partials once into a bf16 h table in shared memory (decode tiles) or build the masked H tiles
 //            themselves (larger tiles); finally the epilogue: tcgen05.ld both accumulators, s_x*s_w*acc0 + acc1, bf16
@@ -48,7 +49,7 @@ struct LoraStep {
 struct K2Ctrl {
     uint64_t full_w[12];
     uint64_t full_b[12];   // B tiles of the expand steps: own barriers, so their consumers need not follow the base phases
-    uint64_t sf_ready[12]; // NVFP4 base: the W slot's scale factors are in tensor memory (and its operands have landed)
+    uint64_t sf_ready[12]; // NVFP4, MXFP4 base: the W slot's scale factors are in tensor memory (and its operands have landed)
     uint64_t empty[12];
     uint64_t empty_b[12];  // release of a slot that held a B tile (4 arrivals: one per expanding warp; 1 from the MMA warp)
     uint64_t h_full[8];
@@ -316,7 +317,7 @@ __device__ __forceinline__ void fused_shrink_units(const K2Params& p, const K1Pa
 
 // EXTRA: the launch adds a residual stream in its stores; every other launch runs an instantiation without that code (a
 // launch's instruction lines are cold fetches after an L2 flush, and the per-element branches lengthen the epilogue).
-template <bool FP4, bool STORED, bool FUSED, bool EXTRA>
+template <int BASE, bool STORED, bool FUSED, bool EXTRA>
 __global__ void __launch_bounds__(kK2Threads, 2)
 k2_kernel(const K2Params p, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
               const __grid_constant__ CUtensorMap tm_b0, const __grid_constant__ CUtensorMap tm_b1,
@@ -324,7 +325,9 @@ k2_kernel(const K2Params p, const __grid_constant__ CUtensorMap tm_w, const __gr
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int tn = p.tn;
-    const int sf_bytes = FP4 ? kSfSlotBytes * (1 + p.nblk) : 0;   // W scales + activation scales of one K slot
+    constexpr bool FP4 = BASE != OB_BASE_FP8, MX = BASE == OB_BASE_MXFP4;
+    constexpr int kSf = sf_slot_bytes(BASE), kAtoms = kSf / 512;  // scale factors of 128 rows x one K slot, in 512-byte atoms
+    const int sf_bytes = FP4 ? kSf * (1 + p.nblk) : 0;            // W scales + activation scales of one K slot
     const int stage_bytes = kWTileBytes + tn * kBlockK + sf_bytes;
     const bool small = tn <= 32;                               // decode tiles: h table in shared memory + a builder warp
     const int nh = p.nh;                                       // masked H tiles in flight
@@ -389,9 +392,9 @@ k2_kernel(const K2Params p, const __grid_constant__ CUtensorMap tm_w, const __gr
         ctrl->last_flag = 0;
         fence_mbar_init();
     }
-    // TMEM: two fp32 accumulators of tn columns; NVFP4 adds, per ring slot, 4 MMAs x (4 columns of W scales + 4 per
-    // 128-token block of activation scales)
-    const uint32_t sf_cols_per_slot = FP4 ? 16u * (1u + (uint32_t)p.nblk) : 0u;
+    // TMEM: two fp32 accumulators of tn columns; NVFP4 and MXFP4 add, per ring slot, 4 or 2 atoms x (4 columns of W scales + 4
+    // per 128-token block of activation scales)
+    const uint32_t sf_cols_per_slot = FP4 ? 4u * kAtoms * (1u + (uint32_t)p.nblk) : 0u;
     uint32_t tmem_used = 2u * (uint32_t)tn + sf_cols_per_slot * (uint32_t)p.stages;
     // Stored adapters on decode tiles: the expand steps' B tiles lie in tensor memory too, rc / 2 columns each -- as many as fit
     // the 256 columns that let two CTAs share an SM, at least one
@@ -456,9 +459,9 @@ k2_kernel(const K2Params p, const __grid_constant__ CUtensorMap tm_w, const __gr
                         uint8_t* slot = ring + (size_t)st * stage_bytes;
                         tma_load_2d(slot + kWTileBytes, &tm_x, &ctrl->full_w[st], (kb0 + r.k) * kBlockK, t0);
                         if (FP4)
-                            bulk_load(slot + kWTileBytes + tn * kBlockK + kSfSlotBytes,
-                                      p.xsf + ((size_t)m_idx * p.kblocks + (kb0 + r.k)) * p.nblk * kSfSlotBytes,
-                                      (uint32_t)(kSfSlotBytes * p.nblk), &ctrl->full_w[st]);
+                            bulk_load(slot + kWTileBytes + tn * kBlockK + kSf,
+                                      p.xsf + ((size_t)m_idx * p.kblocks + (kb0 + r.k)) * p.nblk * kSf,
+                                      (uint32_t)(kSf * p.nblk), &ctrl->full_w[st]);
                     }
                     r.advance(rb, n_base, n_steps);
                 }
@@ -504,14 +507,14 @@ k2_kernel(const K2Params p, const __grid_constant__ CUtensorMap tm_w, const __gr
                     if (w.it == 0) { OB_TRACE(2) }
                     uint8_t* slot = ring + (size_t)st * stage_bytes;
                     if (FP4)
-                        bulk_load(slot + kWTileBytes + tn * kBlockK, p.wsf + ((size_t)n_idx * p.kblocks + (kb0 + w.k)) * kSfSlotBytes,
-                                  kSfSlotBytes, &ctrl->full_w[st]);
+                        bulk_load(slot + kWTileBytes + tn * kBlockK, p.wsf + ((size_t)n_idx * p.kblocks + (kb0 + w.k)) * kSf,
+                                  kSf, &ctrl->full_w[st]);
                     if (k1_done) {
                         tma_load_2d(slot + kWTileBytes, &tm_x, &ctrl->full_w[st], (kb0 + w.k) * kBlockK, t0);
                         if (FP4)
-                            bulk_load(slot + kWTileBytes + tn * kBlockK + kSfSlotBytes,
-                                      p.xsf + ((size_t)m_idx * p.kblocks + (kb0 + w.k)) * p.nblk * kSfSlotBytes,
-                                      (uint32_t)(kSfSlotBytes * p.nblk), &ctrl->full_w[st]);
+                            bulk_load(slot + kWTileBytes + tn * kBlockK + kSf,
+                                      p.xsf + ((size_t)m_idx * p.kblocks + (kb0 + w.k)) * p.nblk * kSf,
+                                      (uint32_t)(kSf * p.nblk), &ctrl->full_w[st]);
                     }
                 }
                 if (++st == p.stages) st = 0;
@@ -594,14 +597,18 @@ k2_kernel(const K2Params p, const __grid_constant__ CUtensorMap tm_w, const __gr
                         const uint32_t sft = tmem_base + 2u * (uint32_t)tn + (uint32_t)st * sf_cols_per_slot;
 #pragma unroll
                         for (int k = 0; k < kBlockK / 32; ++k) {
-                            const uint32_t ta = sft + (uint32_t)k * 4u;
-                            const uint32_t tbs = sft + 16u + (uint32_t)k * 4u * (uint32_t)p.nblk;
-                            if (FUSED) {
+                            const uint32_t at = MX ? (uint32_t)k / 2u : (uint32_t)k;      // the atom that holds the MMA's scales
+                            const uint32_t ta = sft + at * 4u;
+                            const uint32_t tbs = sft + 4u * kAtoms + at * 4u * (uint32_t)p.nblk;
+                            if (FUSED) {                      // (NVFP4: the MXFP4 base has no fused form)
                                 tmem_cp_sf(ta, sf_smem_desc(sfs + (uint32_t)k * 512u));
                                 for (int b = 0; b < p.nblk; ++b)
-                                    tmem_cp_sf(tbs + 4u * (uint32_t)b, sf_smem_desc(sfs + kSfSlotBytes + ((uint32_t)b * 4u + (uint32_t)k) * 512u));
+                                    tmem_cp_sf(tbs + 4u * (uint32_t)b, sf_smem_desc(sfs + kSf + ((uint32_t)b * kAtoms + (uint32_t)k) * 512u));
                             }
-                            umma_nvfp4(acc0, dw + (uint64_t)(k * 2), dx + (uint64_t)(k * 2), idesc4, ta, tbs, k > 0 ? 1u : first);
+                            if (MX)
+                                umma_mxfp4(acc0, dw + (uint64_t)(k * 2), dx + (uint64_t)(k * 2), umma_idesc_mxfp4(kTileN, (uint32_t)tn, (uint32_t)(k & 1) * 2u),
+                                           ta, tbs, k > 0 ? 1u : first);
+                            else umma_nvfp4(acc0, dw + (uint64_t)(k * 2), dx + (uint64_t)(k * 2), idesc4, ta, tbs, k > 0 ? 1u : first);
                         }
                     } else {
 #pragma unroll
@@ -668,7 +675,7 @@ k2_kernel(const K2Params p, const __grid_constant__ CUtensorMap tm_w, const __gr
         }
     } else if (warp == 3) {
         if (FP4 && !FUSED && lane == 0) {
-            // =========================================================== NVFP4: scale copier.  A W slot's scale factors to tensor memory
+            // =========================================================== NVFP4, MXFP4: scale copier.  A W slot's scale factors to tensor memory
             // ahead of its MMAs; a thread of its own because every tcgen05 instruction costs its issuer some 50 cycles and
             // these eight per slot were half of the MMA issuer's time.  It follows every W slot in order.
             SlotWalk w(lead);
@@ -688,11 +695,11 @@ k2_kernel(const K2Params p, const __grid_constant__ CUtensorMap tm_w, const __gr
                     const uint32_t sfs = smem_u32(ring) + (uint32_t)(st * stage_bytes) + kWTileBytes + (uint32_t)tn * kBlockK;
                     const uint32_t sft = tmem_base + 2u * (uint32_t)tn + (uint32_t)st * sf_cols_per_slot;
 #pragma unroll
-                    for (int k = 0; k < kBlockK / 32; ++k) {
+                    for (int k = 0; k < kAtoms; ++k) {
                         tmem_cp_sf(sft + (uint32_t)k * 4u, sf_smem_desc(sfs + (uint32_t)k * 512u));
                         for (int b = 0; b < p.nblk; ++b)
-                            tmem_cp_sf(sft + 16u + ((uint32_t)k * (uint32_t)p.nblk + (uint32_t)b) * 4u,
-                                       sf_smem_desc(sfs + kSfSlotBytes + ((uint32_t)b * 4u + (uint32_t)k) * 512u));
+                            tmem_cp_sf(sft + 4u * kAtoms + ((uint32_t)k * (uint32_t)p.nblk + (uint32_t)b) * 4u,
+                                       sf_smem_desc(sfs + kSf + ((uint32_t)b * kAtoms + (uint32_t)k) * 512u));
                     }
                     umma_commit(&ctrl->sf_ready[st]);
                 }
@@ -1006,7 +1013,7 @@ k2_kernel(const K2Params p, const __grid_constant__ CUtensorMap tm_w, const __gr
         if (done) {
             const bool n_ok = n0_local + n_local < n_s;
             const int n_glob = slice_off + n0_local + n_local;
-            const float s_w = FP4 ? __ldg(p.alpha) : __ldg(p.s_w);   // NVFP4: one scale 1 / (x_global * w_global)
+            const float s_w = FP4 ? __ldg(p.alpha) : __ldg(p.s_w);   // NVFP4: one scale 1 / (x_global * w_global); MXFP4: alpha
             const uint32_t lane_addr = (uint32_t)(q * 32) << 16;
             const bool has_lora = n_steps > 0;
             float* part = p.part + ((size_t)tile_lin * p.split2 + j) * (size_t)tn * kTileN;
@@ -1177,14 +1184,14 @@ k2_kernel(const K2Params p, const __grid_constant__ CUtensorMap tm_w, const __gr
 
 int k2_fp8_h_tiles(int tn) { return tn <= 16 ? 8 : tn <= 32 ? 4 : 2; }
 
-size_t k2_fp8_smem_bytes(int tn, int stages, int rc, int R, int fp4) {
-    const size_t sf = fp4 ? (size_t)kSfSlotBytes * (1 + (tn > 128 ? 2 : 1)) : 0;
+size_t k2_fp8_smem_bytes(int tn, int stages, int rc, int R, int base_fmt) {
+    const size_t sf = (size_t)sf_slot_bytes(base_fmt) * (1 + (tn > 128 ? 2 : 1));
     const size_t aux = (size_t)k2_fp8_h_tiles(tn) * align_up((size_t)tn * rc * 2, 1024) +
                        (tn <= 32 ? align_up((size_t)tn * R * 2, 1024) : 0);
     return 1024 + (size_t)stages * (kWTileBytes + (size_t)tn * kBlockK + sf) + aux + kCtrlBytes;
 }
 
-template <bool FP4, bool STORED, bool FUSED, bool EXTRA = false>
+template <int BASE, bool STORED, bool FUSED, bool EXTRA = false>
 static cudaError_t launch_k2_impl(const K2Params& p, const CUtensorMap& tm_w, const CUtensorMap& tm_x, const CUtensorMap* tm_b,
                                   dim3 grid, size_t smem, int pdl, cudaStream_t stream, const K1Params& k1) {
     static int configured_for[64] = {0};
@@ -1193,9 +1200,9 @@ static cudaError_t launch_k2_impl(const K2Params& p, const CUtensorMap& tm_w, co
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64 && !configured_for[dev]) {
         cudaFuncAttributes fa;                    // the opt-in limit covers static + dynamic shared memory
-        e = cudaFuncGetAttributes(&fa, k2_kernel<FP4, STORED, FUSED, EXTRA>);
+        e = cudaFuncGetAttributes(&fa, k2_kernel<BASE, STORED, FUSED, EXTRA>);
         if (e != cudaSuccess) return e;
-        e = cudaFuncSetAttribute(k2_kernel<FP4, STORED, FUSED, EXTRA>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        e = cudaFuncSetAttribute(k2_kernel<BASE, STORED, FUSED, EXTRA>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  227 * 1024 - (int)fa.sharedSizeBytes);
         if (e != cudaSuccess) return e;
         configured_for[dev] = 1;
@@ -1221,13 +1228,13 @@ static cudaError_t launch_k2_impl(const K2Params& p, const CUtensorMap& tm_w, co
     }
     cfg.attrs = attr;
     cfg.numAttrs = n_attr;
-    return cudaLaunchKernelEx(&cfg, k2_kernel<FP4, STORED, FUSED, EXTRA>, p, tm_w, tm_x, tm_b[0], tm_b[1], tm_b[2], tm_b[3], k1);
+    return cudaLaunchKernelEx(&cfg, k2_kernel<BASE, STORED, FUSED, EXTRA>, p, tm_w, tm_x, tm_b[0], tm_b[1], tm_b[2], tm_b[3], k1);
 }
 
 // How many clusters of `split2` CTAs (grid y) of this kernel the current device keeps resident at once; 0 on error.
-template <bool FP4, bool STORED>
+template <int BASE, bool STORED>
 static int max_clusters_impl(int split2, size_t smem) {
-    cudaError_t e = cudaFuncSetAttribute(k2_kernel<FP4, STORED, false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    cudaError_t e = cudaFuncSetAttribute(k2_kernel<BASE, STORED, false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
     if (e != cudaSuccess) return 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(64, (unsigned)split2, 1);
@@ -1241,41 +1248,43 @@ static int max_clusters_impl(int split2, size_t smem) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int n = 0;
-    e = cudaOccupancyMaxActiveClusters(&n, k2_kernel<FP4, STORED, false, false>, &cfg);
+    e = cudaOccupancyMaxActiveClusters(&n, k2_kernel<BASE, STORED, false, false>, &cfg);
     if (e != cudaSuccess) { (void)cudaGetLastError(); return 0; }
     return n;
 }
 
-int k2_max_active_clusters(int fp4, int stored, int split2, size_t smem) {
-    return fp4 ? (stored ? max_clusters_impl<true, true>(split2, smem) : max_clusters_impl<true, false>(split2, smem))
-               : (stored ? max_clusters_impl<false, true>(split2, smem) : max_clusters_impl<false, false>(split2, smem));
+template <int BASE>
+static int max_clusters_base(int stored, int split2, size_t smem) {
+    return stored ? max_clusters_impl<BASE, true>(split2, smem) : max_clusters_impl<BASE, false>(split2, smem);
+}
+int k2_max_active_clusters(int base_fmt, int stored, int split2, size_t smem) {
+    return base_fmt == OB_BASE_NVFP4   ? max_clusters_base<OB_BASE_NVFP4>(stored, split2, smem)
+           : base_fmt == OB_BASE_MXFP4 ? max_clusters_base<OB_BASE_MXFP4>(stored, split2, smem)
+                                       : max_clusters_base<OB_BASE_FP8>(stored, split2, smem);
 }
 
-cudaError_t launch_k2_fp8(const K2Params& p, const CUtensorMap& tm_w, const CUtensorMap& tm_x, const CUtensorMap* tm_b,
-                          dim3 grid, size_t smem, int pdl, cudaStream_t stream) {
+template <int BASE>
+static cudaError_t launch_k2_base(const K2Params& p, const CUtensorMap& tm_w, const CUtensorMap& tm_x, const CUtensorMap* tm_b,
+                                  dim3 grid, size_t smem, int pdl, cudaStream_t stream) {
     const K1Params none = {};
     if (p.residual != nullptr)
-        return p.lora_fmt == kLoraBf16 ? launch_k2_impl<false, false, false, true>(p, tm_w, tm_x, tm_b, grid, smem, pdl, stream, none)
-                                       : launch_k2_impl<false, true, false, true>(p, tm_w, tm_x, tm_b, grid, smem, pdl, stream, none);
-    return p.lora_fmt == kLoraBf16 ? launch_k2_impl<false, false, false>(p, tm_w, tm_x, tm_b, grid, smem, pdl, stream, none)
-                                   : launch_k2_impl<false, true, false>(p, tm_w, tm_x, tm_b, grid, smem, pdl, stream, none);
+        return p.lora_fmt == kLoraBf16 ? launch_k2_impl<BASE, false, false, true>(p, tm_w, tm_x, tm_b, grid, smem, pdl, stream, none)
+                                       : launch_k2_impl<BASE, true, false, true>(p, tm_w, tm_x, tm_b, grid, smem, pdl, stream, none);
+    return p.lora_fmt == kLoraBf16 ? launch_k2_impl<BASE, false, false>(p, tm_w, tm_x, tm_b, grid, smem, pdl, stream, none)
+                                   : launch_k2_impl<BASE, true, false>(p, tm_w, tm_x, tm_b, grid, smem, pdl, stream, none);
 }
-
-cudaError_t launch_k2_nvfp4(const K2Params& p, const CUtensorMap& tm_w, const CUtensorMap& tm_x, const CUtensorMap* tm_b,
-                            dim3 grid, size_t smem, int pdl, cudaStream_t stream) {
-    const K1Params none = {};
-    if (p.residual != nullptr)
-        return p.lora_fmt == kLoraBf16 ? launch_k2_impl<true, false, false, true>(p, tm_w, tm_x, tm_b, grid, smem, pdl, stream, none)
-                                       : launch_k2_impl<true, true, false, true>(p, tm_w, tm_x, tm_b, grid, smem, pdl, stream, none);
-    return p.lora_fmt == kLoraBf16 ? launch_k2_impl<true, false, false>(p, tm_w, tm_x, tm_b, grid, smem, pdl, stream, none)
-                                   : launch_k2_impl<true, true, false>(p, tm_w, tm_x, tm_b, grid, smem, pdl, stream, none);
+cudaError_t launch_k2(int base_fmt, const K2Params& p, const CUtensorMap& tm_w, const CUtensorMap& tm_x, const CUtensorMap* tm_b,
+                      dim3 grid, size_t smem, int pdl, cudaStream_t stream) {
+    return base_fmt == OB_BASE_NVFP4   ? launch_k2_base<OB_BASE_NVFP4>(p, tm_w, tm_x, tm_b, grid, smem, pdl, stream)
+           : base_fmt == OB_BASE_MXFP4 ? launch_k2_base<OB_BASE_MXFP4>(p, tm_w, tm_x, tm_b, grid, smem, pdl, stream)
+                                       : launch_k2_base<OB_BASE_FP8>(p, tm_w, tm_x, tm_b, grid, smem, pdl, stream);
 }
 
 // The fused decode kernel (bf16 adapters, one token tile of at most 32 tokens): quantization, shrink and GEMM in one launch.
 cudaError_t launch_fused(const K2Params& p, const K1Params& k1, const CUtensorMap& tm_w, const CUtensorMap& tm_x,
                          const CUtensorMap* tm_b, dim3 grid, size_t smem, cudaStream_t stream) {
-    return k1.base_fmt == OB_BASE_NVFP4 ? launch_k2_impl<true, false, true>(p, tm_w, tm_x, tm_b, grid, smem, 1, stream, k1)
-                                        : launch_k2_impl<false, false, true>(p, tm_w, tm_x, tm_b, grid, smem, 1, stream, k1);
+    return k1.base_fmt == OB_BASE_NVFP4 ? launch_k2_impl<OB_BASE_NVFP4, false, true>(p, tm_w, tm_x, tm_b, grid, smem, 1, stream, k1)
+                                        : launch_k2_impl<OB_BASE_FP8, false, true>(p, tm_w, tm_x, tm_b, grid, smem, 1, stream, k1);
 }
 
 }  // namespace ob

@@ -5,6 +5,9 @@
 // and its columns are consecutive features -- a thread of the epilogue stores 64 contiguous bytes of a row of y per
 // tensor-memory load).
 //
+// An MXFP4 base runs the NVFP4 form with kind::mxf4 and half of the scale bytes: two atoms per 128 rows and slot, each of which
+// serves two MMAs.
+//
 // Why pairs: a ring slot costs its single-thread roles a fixed time (every wait, copy issue, tcgen05.cp / mma / commit costs
 // its issuing thread 50-250 cycles), whatever the slot holds.  In a pair each CTA supplies its own 128 rows of W per 256
 // features and only HALF of the token tile (the MMA reads the other half out of the partner's shared memory), so a CTA takes
@@ -57,14 +60,15 @@ static_assert(2 * kP2RegsRoles + 2 * kP2RegsEpilogue <= 4 * 128, "register split
 constexpr int kP2Tokens = 256;               // tokens per tile: 128 per CTA (the MMA's M)
 constexpr int kP2WBytes = 128 * 128;         // 128 rows of W (or B_l) of a slot
 constexpr int kP2XBytes = 128 * 128;         // this CTA's half of the token tile
-constexpr int kP2SfCols = 48;                // NVFP4: tensor-memory columns of one slot's scale factors (16 tokens' + 32 W)
+// NVFP4, MXFP4: tensor-memory columns of one slot's scale factors (four per atom: the tokens' atoms, then twice as many of W)
+__host__ __device__ constexpr int p2_sf_cols(int base_fmt) { return 3 * 4 * (sf_slot_bytes(base_fmt) / 512); }
 constexpr int kP2MaxSteps = 512;
-// Ring depth and slot size of a tile of `halves` 256-feature halves (NVFP4: one N = 256 MMA; FP8: one or two -- two take all
+// Ring depth and slot size of a tile of `halves` 256-feature halves (NVFP4, MXFP4: one N = 256 MMA; FP8: one or two -- two take all
 // 512 accumulator columns, with one the accumulators are double-buffered)
 constexpr int kP2MaxStages = 6;
-__host__ __device__ constexpr int p2_stages(bool fp4, int halves) { return fp4 ? 5 : halves == 2 ? 4 : 6; }
-__host__ __device__ constexpr int p2_slot_bytes(bool fp4, int halves) {
-    return halves * kP2WBytes + kP2XBytes + (fp4 ? 3 * kSfSlotBytes : 0);   // 38 KB / 48 KB or 32 KB
+__host__ __device__ constexpr int p2_stages(int base_fmt, int halves) { return base_fmt != OB_BASE_FP8 ? 5 : halves == 2 ? 4 : 6; }
+__host__ __device__ constexpr int p2_slot_bytes(int base_fmt, int halves) {
+    return halves * kP2WBytes + kP2XBytes + 3 * sf_slot_bytes(base_fmt);    // 38 KB (NVFP4), 35 KB (MXFP4), 48 KB or 32 KB
 }
 
 constexpr uint16_t kP2NoEntry = 0xFFFFu;
@@ -182,7 +186,7 @@ struct P2Walk {
 // EXTRA: the launch adds a residual stream in its stores; every other launch runs an instantiation without that code.  The
 // residual's pieces are asked into L2 under the main loop and loaded just before the step's transposes.  down at 2048 tokens with SiLU * mul
 // and residual, whole projection: 458 us (128-token tiles of k2_gemm.cu, the transform evaluated three times) -> 197 us.
-template <bool FP4, int HALVES, bool EXTRA, bool STORED>
+template <int BASE, int HALVES, bool EXTRA, bool STORED>
 __global__ void __launch_bounds__(kP2Threads, 1)
 k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
                        const __grid_constant__ CUtensorMap tm_h, const __grid_constant__ CUtensorMap tm_b0,
@@ -192,7 +196,9 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
     extern __shared__ uint8_t smem_raw[];
     // (the dynamic shared memory starts at the same offset in both CTAs of a pair: the MMA applies one descriptor to both)
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    constexpr int kHalves = HALVES, kRows = 256 * HALVES, kStages = p2_stages(FP4, HALVES), kSlot = p2_slot_bytes(FP4, HALVES);
+    constexpr bool FP4 = BASE != OB_BASE_FP8, MX = BASE == OB_BASE_MXFP4;
+    constexpr int kSf = sf_slot_bytes(BASE), kAtoms = kSf / 512, kSfCols = p2_sf_cols(BASE);
+    constexpr int kHalves = HALVES, kRows = 256 * HALVES, kStages = p2_stages(BASE, HALVES), kSlot = p2_slot_bytes(BASE, HALVES);
     constexpr int kAccBufs = !FP4 && HALVES == 1 ? 2 : 1;     // (NVFP4: the scale factors take the rest of tensor memory)
     constexpr int kXOff = kHalves * kP2WBytes;                // the token tile (or h block) follows the W (or B_l) rows in a slot
     uint8_t* ring = smem;
@@ -288,13 +294,13 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
                             tma_load_2d_pair(slot + h * kP2WBytes, &tm_w, bar0, kb * 128, tl.slice_off + row0 + h * 256);
                         tma_load_2d_pair(slot + kXOff, &tm_x, bar0, kb * 128, tl.t0 + (int)rank * 128);
                         if (FP4) {
-                            // scales, as 8 x 256-byte rows of a [rows, 256] byte tensor per 2 KB atom: this CTA's 128 tokens (the
+                            // scales, as 8 (MXFP4: 4) x 256-byte rows of a [rows, 256] byte tensor: this CTA's 128 tokens (the
                             // MMA's A rows), then both 128-feature tiles of W (every CTA needs the scales of all of B's 256 rows in
                             // its own tensor memory)
                             uint8_t* sf = slot + kXOff + kP2XBytes;
-                            tma_load_2d_pair(sf, &tm_xsf, bar0, 0, ((tl.m_idx * p.kblocks + kb) * 2 + (int)rank) * 8);
-                            tma_load_2d_pair(sf + kSfSlotBytes, &tm_wsf, bar0, 0, (tl.sf_tile * p.kblocks + kb) * 8);
-                            tma_load_2d_pair(sf + 2 * kSfSlotBytes, &tm_wsf, bar0, 0, ((tl.sf_tile + 1) * p.kblocks + kb) * 8);
+                            tma_load_2d_pair(sf, &tm_xsf, bar0, 0, ((tl.m_idx * p.kblocks + kb) * 2 + (int)rank) * (kSf / 256));
+                            tma_load_2d_pair(sf + kSf, &tm_wsf, bar0, 0, (tl.sf_tile * p.kblocks + kb) * (kSf / 256));
+                            tma_load_2d_pair(sf + 2 * kSf, &tm_wsf, bar0, 0, ((tl.sf_tile + 1) * p.kblocks + kb) * (kSf / 256));
                         }
                         ++kb;
                     } else {
@@ -357,11 +363,15 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
                     tc_fence_after();
                     const uint64_t off = (uint64_t)(uint32_t)(st * (kSlot >> 4));
                     const uint64_t dx = d_x0 + off, dw = d_w0 + off;
-                    const uint32_t sft = tmem_base + 256u + (uint32_t)(st * kP2SfCols);
+                    const uint32_t sft = tmem_base + 256u + (uint32_t)(st * kSfCols);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const uint32_t ta = sft + (uint32_t)k * 4u, tb = sft + 16u + (uint32_t)k * 8u;
-                        umma_nvfp4_pair(acc, dx + (uint64_t)(k * 2), dw + (uint64_t)(k * 2), idesc4, ta, tb, k > 0 ? 1u : first);
+                        const uint32_t at = MX ? (uint32_t)k / 2u : (uint32_t)k;          // the atom that holds the MMA's scales
+                        const uint32_t ta = sft + at * 4u, tb = sft + 4u * kAtoms + at * 8u;
+                        if (MX)
+                            umma_mxfp4_pair(acc, dx + (uint64_t)(k * 2), dw + (uint64_t)(k * 2), umma_idesc_mxfp4(256, 256, (uint32_t)(k & 1) * 2u), ta,
+                                            tb, k > 0 ? 1u : first);
+                        else umma_nvfp4_pair(acc, dx + (uint64_t)(k * 2), dw + (uint64_t)(k * 2), idesc4, ta, tb, k > 0 ? 1u : first);
                     }
                 } else {
                     if (!p2_wait<true>(p, ctrl, &ctrl->full[st], ph, limit_ns, 4, it)) return false;
@@ -464,11 +474,11 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
             }
         }
     } else if (warp == 3 || warp >= 12) {
-        // =========================================================== scale copiers (NVFP4, rank 0; warps 3, 12, 13): a k-block
+        // =========================================================== scale copiers (NVFP4, MXFP4, rank 0; warps 3, 12, 13): a k-block
         // slot's scale factors -> both CTAs' tensor memory, ahead of the MMAs.  Threads of their own because every tcgen05
         // instruction costs its issuer some 50 cycles: twelve copies per slot from one thread (with its wait and commit, 920
         // cycles) bounded the main loop, whose four MMAs take the tensor pipe some 540.  Copier 0 moves the tokens' scales,
-        // copiers 1 and 2 those of the two 128-feature halves of W: four copies each per slot.
+        // copiers 1 and 2 those of the two 128-feature halves of W: four copies (MXFP4: two) each per slot.
         const int cpi = warp == 3 ? 0 : warp - 11;
         if (FP4 && lane == 0 && rank == 0 && cpi < 3) {
             int it = 0, st = 0;
@@ -495,11 +505,11 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
                     if (!step) {
                         tc_fence_after();
                         const uint32_t sfs = smem_u32(ring + (size_t)st * kSlot) + (uint32_t)(kXOff + kP2XBytes);
-                        const uint32_t sft = tmem_base + 256u + (uint32_t)(st * kP2SfCols);
+                        const uint32_t sft = tmem_base + 256u + (uint32_t)(st * kSfCols);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const uint32_t dst = cpi == 0 ? sft + (uint32_t)k * 4u : sft + 16u + (uint32_t)k * 8u + (uint32_t)(cpi - 1) * 4u;
-                            tmem_cp_sf_pair(dst, sf_smem_desc(sfs + (uint32_t)cpi * kSfSlotBytes + (uint32_t)k * 512u));
+                        for (int k = 0; k < kAtoms; ++k) {
+                            const uint32_t dst = cpi == 0 ? sft + (uint32_t)k * 4u : sft + 4u * kAtoms + (uint32_t)k * 8u + (uint32_t)(cpi - 1) * 4u;
+                            tmem_cp_sf_pair(dst, sf_smem_desc(sfs + (uint32_t)(cpi * kSf) + (uint32_t)k * 512u));
                         }
                         umma_commit_pair(&ctrl->sf_ready[st], 1);      // (arrives in rank 0 only)
                     }
@@ -806,12 +816,12 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
     }
 }
 
-template <bool FP4, int HALVES>
+template <int BASE, int HALVES>
 static void pair_launch_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr, int pairs, int pdl, cudaStream_t stream) {
     *cfg = cudaLaunchConfig_t{};
     cfg->gridDim = dim3((unsigned)(2 * pairs));
     cfg->blockDim = dim3(kP2Threads);
-    cfg->dynamicSmemBytes = 1024 + (size_t)p2_stages(FP4, HALVES) * (size_t)p2_slot_bytes(FP4, HALVES) + sizeof(P2Ctrl) + 64;
+    cfg->dynamicSmemBytes = 1024 + (size_t)p2_stages(BASE, HALVES) * (size_t)p2_slot_bytes(BASE, HALVES) + sizeof(P2Ctrl) + 64;
     cfg->stream = stream;
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2;
@@ -834,20 +844,20 @@ int k2_prefill_pair_capacity() {
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { (void)cudaGetLastError(); return 0; }
     int n = cached[dev].load();
     if (n > 0) return n;
-    if (cudaFuncSetAttribute(k2_prefill_pair_kernel<false, 2, false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024) != cudaSuccess) {
+    if (cudaFuncSetAttribute(k2_prefill_pair_kernel<OB_BASE_FP8, 2, false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024) != cudaSuccess) {
         (void)cudaGetLastError();
         return 0;
     }
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attr[2];
-    pair_launch_config<false, 2>(&cfg, attr, 148, 0, nullptr);
+    pair_launch_config<OB_BASE_FP8, 2>(&cfg, attr, 148, 0, nullptr);
     n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, k2_prefill_pair_kernel<false, 2, false, false>, &cfg) != cudaSuccess) { (void)cudaGetLastError(); return 0; }
+    if (cudaOccupancyMaxActiveClusters(&n, k2_prefill_pair_kernel<OB_BASE_FP8, 2, false, false>, &cfg) != cudaSuccess) { (void)cudaGetLastError(); return 0; }
     cached[dev].store(n);
     return n;
 }
 
-template <bool FP4, int HALVES, bool EXTRA, bool STORED>
+template <int BASE, int HALVES, bool EXTRA, bool STORED>
 static cudaError_t launch_pair_impl(const K2pParams& p, const CUtensorMap& tm_w, const CUtensorMap& tm_x, const CUtensorMap& tm_h,
                                     const CUtensorMap* tm_b, const CUtensorMap* tm_sf, int pairs, int pdl, cudaStream_t stream) {
     static std::atomic<unsigned long long> configured{0};     // devices whose limit on dynamic shared memory was raised
@@ -858,39 +868,40 @@ static cudaError_t launch_pair_impl(const K2pParams& p, const CUtensorMap& tm_w,
         // the epilogue's warps wait for the registers the others give back: a build that launched with fewer than the split adds
         // up to would wait for good, so it is refused here
         cudaFuncAttributes fa;
-        e = cudaFuncGetAttributes(&fa, k2_prefill_pair_kernel<FP4, HALVES, EXTRA, STORED>);
+        e = cudaFuncGetAttributes(&fa, k2_prefill_pair_kernel<BASE, HALVES, EXTRA, STORED>);
         if (e != cudaSuccess) return e;
         if (fa.numRegs * 4 < 2 * kP2RegsRoles + 2 * kP2RegsEpilogue) return cudaErrorLaunchOutOfResources;
-        e = cudaFuncSetAttribute(k2_prefill_pair_kernel<FP4, HALVES, EXTRA, STORED>, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
+        e = cudaFuncSetAttribute(k2_prefill_pair_kernel<BASE, HALVES, EXTRA, STORED>, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
         if (e != cudaSuccess) return e;
         configured.fetch_or(1ull << dev);
     }
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attr[2];
-    pair_launch_config<FP4, HALVES>(&cfg, attr, pairs, pdl, stream);
-    return cudaLaunchKernelEx(&cfg, k2_prefill_pair_kernel<FP4, HALVES, EXTRA, STORED>, p, tm_w, tm_x, tm_h, tm_b[0], tm_b[1], tm_b[2],
-                              tm_b[3], FP4 ? tm_sf[0] : tm_w, FP4 ? tm_sf[1] : tm_w);
+    pair_launch_config<BASE, HALVES>(&cfg, attr, pairs, pdl, stream);
+    return cudaLaunchKernelEx(&cfg, k2_prefill_pair_kernel<BASE, HALVES, EXTRA, STORED>, p, tm_w, tm_x, tm_h, tm_b[0], tm_b[1], tm_b[2],
+                              tm_b[3], BASE != OB_BASE_FP8 ? tm_sf[0] : tm_w, BASE != OB_BASE_FP8 ? tm_sf[1] : tm_w);
 }
 
 template <bool EXTRA, bool STORED>
 static cudaError_t launch_pair_form(const K2pParams& p, const CUtensorMap& tm_w, const CUtensorMap& tm_x, const CUtensorMap& tm_h,
-                                    const CUtensorMap* tm_b, const CUtensorMap* tm_sf, int pairs, int fp4, int halves, int pdl,
+                                    const CUtensorMap* tm_b, const CUtensorMap* tm_sf, int pairs, int base_fmt, int halves, int pdl,
                                     cudaStream_t stream) {
-    return fp4           ? launch_pair_impl<true, 1, EXTRA, STORED>(p, tm_w, tm_x, tm_h, tm_b, tm_sf, pairs, pdl, stream)
-           : halves == 1 ? launch_pair_impl<false, 1, EXTRA, STORED>(p, tm_w, tm_x, tm_h, tm_b, tm_sf, pairs, pdl, stream)
-                         : launch_pair_impl<false, 2, EXTRA, STORED>(p, tm_w, tm_x, tm_h, tm_b, tm_sf, pairs, pdl, stream);
+    return base_fmt == OB_BASE_NVFP4   ? launch_pair_impl<OB_BASE_NVFP4, 1, EXTRA, STORED>(p, tm_w, tm_x, tm_h, tm_b, tm_sf, pairs, pdl, stream)
+           : base_fmt == OB_BASE_MXFP4 ? launch_pair_impl<OB_BASE_MXFP4, 1, EXTRA, STORED>(p, tm_w, tm_x, tm_h, tm_b, tm_sf, pairs, pdl, stream)
+           : halves == 1               ? launch_pair_impl<OB_BASE_FP8, 1, EXTRA, STORED>(p, tm_w, tm_x, tm_h, tm_b, tm_sf, pairs, pdl, stream)
+                                       : launch_pair_impl<OB_BASE_FP8, 2, EXTRA, STORED>(p, tm_w, tm_x, tm_h, tm_b, tm_sf, pairs, pdl, stream);
 }
 
-// tm_sf: NVFP4 base only, the packed W block scales and the workspace's token block scales as [rows, 256] byte tensors
+// tm_sf: NVFP4 and MXFP4 base only, the packed W block scales and the workspace's token block scales as [rows, 256] byte tensors
 cudaError_t launch_k2_prefill_pair(const K2pParams& p, const CUtensorMap& tm_w, const CUtensorMap& tm_x, const CUtensorMap& tm_h,
-                                   const CUtensorMap* tm_b, const CUtensorMap* tm_sf, int pairs, int fp4, int halves, int pdl,
+                                   const CUtensorMap* tm_b, const CUtensorMap* tm_sf, int pairs, int base_fmt, int halves, int pdl,
                                    cudaStream_t stream) {
     const bool extra = p.residual != nullptr, stored = p.lora_fmt != kLoraBf16;
     if (extra)
-        return stored ? launch_pair_form<true, true>(p, tm_w, tm_x, tm_h, tm_b, tm_sf, pairs, fp4, halves, pdl, stream)
-                      : launch_pair_form<true, false>(p, tm_w, tm_x, tm_h, tm_b, tm_sf, pairs, fp4, halves, pdl, stream);
-    return stored ? launch_pair_form<false, true>(p, tm_w, tm_x, tm_h, tm_b, tm_sf, pairs, fp4, halves, pdl, stream)
-                  : launch_pair_form<false, false>(p, tm_w, tm_x, tm_h, tm_b, tm_sf, pairs, fp4, halves, pdl, stream);
+        return stored ? launch_pair_form<true, true>(p, tm_w, tm_x, tm_h, tm_b, tm_sf, pairs, base_fmt, halves, pdl, stream)
+                      : launch_pair_form<true, false>(p, tm_w, tm_x, tm_h, tm_b, tm_sf, pairs, base_fmt, halves, pdl, stream);
+    return stored ? launch_pair_form<false, true>(p, tm_w, tm_x, tm_h, tm_b, tm_sf, pairs, base_fmt, halves, pdl, stream)
+                  : launch_pair_form<false, false>(p, tm_w, tm_x, tm_h, tm_b, tm_sf, pairs, base_fmt, halves, pdl, stream);
 }
 
 }  // namespace ob

@@ -11,14 +11,14 @@
 #include "ob_common.cuh"
 
 namespace ob {
-size_t k2_fp8_smem_bytes(int tn, int stages, int rc, int R, int fp4);
-cudaError_t launch_k2_nvfp4(const K2Params& p, const CUtensorMap& tm_w, const CUtensorMap& tm_x, const CUtensorMap* tm_b,
-                            dim3 grid, size_t smem, int pdl, cudaStream_t stream);
+size_t k2_fp8_smem_bytes(int tn, int stages, int rc, int R, int base_fmt);
+cudaError_t launch_k2(int base_fmt, const K2Params& p, const CUtensorMap& tm_w, const CUtensorMap& tm_x, const CUtensorMap* tm_b,
+                      dim3 grid, size_t smem, int pdl, cudaStream_t stream);
 int k2_fp8_h_tiles(int tn);
-int k2_max_active_clusters(int fp4, int stored, int split2, size_t smem);
+int k2_max_active_clusters(int base_fmt, int stored, int split2, size_t smem);
 cudaError_t launch_k1_mma(const K1mParams& p, const CUtensorMap& tm_xs, const CUtensorMap* tm_a, dim3 grid, cudaStream_t stream);
 cudaError_t launch_k2_prefill_pair(const K2pParams& p, const CUtensorMap& tm_w, const CUtensorMap& tm_x, const CUtensorMap& tm_h,
-                                   const CUtensorMap* tm_b, const CUtensorMap* tm_sf, int pairs, int fp4, int halves, int pdl,
+                                   const CUtensorMap* tm_b, const CUtensorMap* tm_sf, int pairs, int base_fmt, int halves, int pdl,
                                    cudaStream_t stream);
 int k2_prefill_pair_capacity();
 int k2_prefill_pair_max_steps();
@@ -29,13 +29,11 @@ cudaError_t launch_requant_nvfp4(const void* src, int l, int rows, int cols, voi
 cudaError_t launch_fused(const K2Params& p, const K1Params& k1, const CUtensorMap& tm_w, const CUtensorMap& tm_x,
                          const CUtensorMap* tm_b, dim3 grid, size_t smem, cudaStream_t stream);
 cudaError_t launch_k1_fp8(const K1Params& p, int grid, int pdl, cudaStream_t stream);
-cudaError_t launch_k2_fp8(const K2Params& p, const CUtensorMap& tm_w, const CUtensorMap& tm_x, const CUtensorMap* tm_b,
-                          dim3 grid, size_t smem, int pdl, cudaStream_t stream);
 size_t k2_stream_smem_bytes(int tn, int stages, int rc, int R, int S, int fp4);
 int k2_stream_h_tiles(int tn);
 cudaError_t launch_k2_stream(const K2Params& p, const CUtensorMap& tm_w, const CUtensorMap& tm_x, const CUtensorMap* tm_b,
                              int grid, size_t smem, int fp4, int pdl, cudaStream_t stream);
-cudaError_t launch_pack_scales(const uint8_t* linear, int K, int S, const int32_t* widths, uint8_t* packed, size_t bytes,
+cudaError_t launch_pack_scales(int base_fmt, const uint8_t* linear, int K, int S, const int32_t* widths, uint8_t* packed, size_t bytes,
                                cudaStream_t stream);
 cudaError_t launch_rms_norm(const ObRmsNorm& p, cudaStream_t stream);
 cudaError_t launch_mxfp4_quantize(const void* x, int dtype, long long rows, int K, long long ldx, void* codes, void* scales, cudaStream_t stream);
@@ -130,16 +128,18 @@ struct ObLayer {
     CUtensorMap tm_b[OB_MAX_SLICES];
     CUtensorMap tm_a[OB_MAX_SLICES];   // bf16 adapters: A of each slice as [L * R, K], for the tensor-core shrink
     bool big_ok;                       // the large-tile prefill GEMM applies (see ob_layer_create)
-    CUtensorMap tm_wsf;                //   NVFP4 base: the packed W block scales as a [rows, 256] byte tensor (8 rows per atom)
+    CUtensorMap tm_wsf;                //   NVFP4, MXFP4 base: the packed W block scales as a [rows, 256] byte tensor
     std::mutex mu;
     std::vector<XMap> xmaps;      // x_q maps by (workspace region, rows, token tile)
 };
 
 namespace {
 
+bool is_fp4(const ObLayerDesc& d) { return d.base_fmt == OB_BASE_NVFP4 || d.base_fmt == OB_BASE_MXFP4; }
+
 int validate_desc(const ObLayerDesc* d) {
     if (!d) return OB_ERR_NULL;
-    if (d->base_fmt != OB_BASE_FP8 && d->base_fmt != OB_BASE_NVFP4) return OB_ERR_FORMAT;
+    if (d->base_fmt != OB_BASE_FP8 && !is_fp4(*d)) return OB_ERR_FORMAT;
     if (d->lora_fmt != OB_LORA_BF16 && d->lora_fmt != OB_LORA_FP8 && d->lora_fmt != OB_LORA_NVFP4) return OB_ERR_FORMAT;
     if (d->N <= 0 || d->K <= 0 || d->K % 16 != 0 || d->S < 1 || d->S > OB_MAX_SLICES || d->L < 1 || d->L > 256 ||
         d->max_m < 1)
@@ -154,7 +154,8 @@ int validate_desc(const ObLayerDesc* d) {
     if (!d->w_q) return OB_ERR_NULL;
     if (d->base_fmt == OB_BASE_FP8 && !d->s_w) return OB_ERR_NULL;
     if (d->base_fmt == OB_BASE_NVFP4 && (!d->w_sf || !d->x_global || !d->alpha)) return OB_ERR_NULL;
-    if (d->base_fmt == OB_BASE_NVFP4 && d->K % 32 != 0) return OB_ERR_SHAPE;
+    if (d->base_fmt == OB_BASE_MXFP4 && (!d->w_sf || !d->alpha)) return OB_ERR_NULL;
+    if (is_fp4(*d) && d->K % 32 != 0) return OB_ERR_SHAPE;
     if (!aligned16(d->w_q) || (d->w_sf && !aligned16(d->w_sf))) return OB_ERR_ALIGN;
     for (int s = 0; s < d->S; ++s) {
         if (!d->a[s] || !d->b[s]) return OB_ERR_NULL;
@@ -182,7 +183,12 @@ int validate_batch(const ObLayer* l, const ObBatch* b) {
     if (!l || !b) return OB_ERR_NULL;
     if (b->M < 1 || b->M > l->d.max_m) return OB_ERR_BATCH;
     if (!b->x || !b->y || !b->tok || !b->srt || !b->seg_n || !b->seg_start || !b->seg_ids) return OB_ERR_NULL;
-    if (b->x_op != OB_X_PLAIN && b->x_op != OB_X_SILU_MUL) return OB_ERR_FORMAT;
+    if (b->x_op != OB_X_PLAIN && b->x_op != OB_X_SILU_MUL && b->x_op != OB_X_QUANTIZED) return OB_ERR_FORMAT;
+    if (b->x_op == OB_X_QUANTIZED) {
+        if (l->d.base_fmt == OB_BASE_NVFP4) return OB_ERR_FORMAT;
+        if (!b->x_codes || !b->x_scales) return OB_ERR_NULL;
+        if (!aligned16(b->x_codes) || (l->d.base_fmt == OB_BASE_FP8 && (reinterpret_cast<uintptr_t>(b->x_scales) & 3u))) return OB_ERR_ALIGN;
+    }
     if (!aligned16(b->x) || b->ldx < (b->x_op == OB_X_SILU_MUL ? 2 : 1) * (int64_t)l->d.K || b->ldx % 8 != 0) return OB_ERR_ALIGN;
     if (b->residual && ((reinterpret_cast<uintptr_t>(b->residual) & 1u) || b->ldr < l->d.N)) return OB_ERR_ALIGN;
     if ((reinterpret_cast<uintptr_t>(b->y) & 1u) || b->ldy < l->d.N) return OB_ERR_ALIGN;
@@ -198,7 +204,7 @@ int validate_workspace(const ObLayer* l, const void* ws, const ObWorkspaceShape*
     return OB_OK;
 }
 
-int k_bytes(const ObLayerDesc& d) { return d.base_fmt == OB_BASE_NVFP4 ? d.K / 2 : d.K; }
+int k_bytes(const ObLayerDesc& d) { return is_fp4(d) ? d.K / 2 : d.K; }
 
 struct Resolved {
     int tn, split1, split2, stages, m_tiles, k_per_split, pb, fused, mma_shrink, big;
@@ -265,7 +271,7 @@ long long shrink_items(const ObLayerDesc& d, int M) {
 // tokens, 3 of rank 16 52 -> 48, 2 of rank 128 69 -> 83, 6 of rank 256 181 -> 144; 200 tokens, 4 of rank 128 98 -> 81.
 bool small_tiles_win(const ObLayerDesc& d, int m_tiles, long long big_tiles) {
     const long long n = big_tiles / m_tiles;             // 256-feature tiles of one token tile
-    const bool fp4 = d.base_fmt == OB_BASE_NVFP4, fp8_stored = d.lora_fmt == OB_LORA_FP8, stored = d.lora_fmt != OB_LORA_BF16;
+    const bool fp4 = is_fp4(d), fp8_stored = d.lora_fmt == OB_LORA_FP8, stored = d.lora_fmt != OB_LORA_BF16;
     if (d.K > 4096 || m_tiles > 2 || d.L > 8) return false;
     if (d.S == 1 && d.R >= 128 && d.L >= 3) {
         if (fp4) return n <= 16 && (stored ? m_tiles == 1 || fp8_stored : m_tiles == 1 && d.R == 256 && d.L <= 6);
@@ -282,10 +288,10 @@ bool small_tiles_win(const ObLayerDesc& d, int m_tiles, long long big_tiles) {
 // `call_takes_big`: nothing about the call's own tensors and workspace rules the large tiles out (see call_takes_big()).
 int resolve_cfg(const ObLayer* l, int M, const ObTileCfg* cfg, Resolved* r, int max_split1 = 32, bool call_takes_big = true) {
     const ObLayerDesc& d = l->d;
-    const bool fp4 = d.base_fmt == OB_BASE_NVFP4;
+    const bool fp4 = is_fp4(d);
     const int kblocks = (k_bytes(d) + kBlockK - 1) / kBlockK;
     r->tn = (cfg && cfg->tn) ? cfg->tn : default_tn(M);
-    // NVFP4: the scale factors share tensor memory with the accumulators; 64-token tiles leave room for two CTAs per SM
+    // NVFP4, MXFP4: the scale factors share tensor memory with the accumulators; 64-token tiles leave room for two CTAs per SM
     if (fp4 && r->tn > 64 && !(cfg && cfg->tn)) r->tn = 64;
     if (fp4 && r->tn > 128) return OB_ERR_TILE;   // (the large-tile prefill GEMM has its own 256-token tile: `big` below)
     if (!(r->tn == 16 || r->tn == 32 || r->tn == 64 || r->tn == 128 || r->tn == 256)) return OB_ERR_TILE;
@@ -301,7 +307,7 @@ int resolve_cfg(const ObLayer* l, int M, const ObTileCfg* cfg, Resolved* r, int 
         const int want = cfg ? cfg->stream : 0;
         const int sms = sm_count();
         const long long units = (long long)l->n_tiles * kblocks;
-        if ((want == 1 || (env_stream && want != 2)) && !(cfg && cfg->fused) && sms > 0 &&
+        if ((want == 1 || (env_stream && want != 2)) && !(cfg && cfg->fused) && sms > 0 && d.base_fmt != OB_BASE_MXFP4 &&
             M <= kDecodeTokens && r->tn <= 32 && r->m_tiles == 1 && d.lora_fmt == kLoraBf16 && l->n_tiles <= kCounterSlots &&
             (long long)(d.L < r->tn ? d.L : r->tn) * (d.R / l->rc) <= 256) {
             // Ring depth: measured on a B200, the stream rate does not grow beyond 4-6 slots (HBM, not latency, bounds it), and
@@ -395,18 +401,18 @@ int resolve_cfg(const ObLayer* l, int M, const ObTileCfg* cfg, Resolved* r, int 
     if (stages == 0) {   // prefer a footprint that lets two CTAs share an SM (3+ stages; 2+ for 128-token tiles), else the deepest ring that fits
         stages = 12;
         const int floor_stages = r->tn >= 128 ? 2 : 3;
-        while (stages > floor_stages && k2_fp8_smem_bytes(r->tn, stages, rc, d.R, fp4 ? 1 : 0) > kSmemTwoPerSm) --stages;
-        if (k2_fp8_smem_bytes(r->tn, stages, rc, d.R, fp4 ? 1 : 0) > kSmemTwoPerSm) stages = 12;
+        while (stages > floor_stages && k2_fp8_smem_bytes(r->tn, stages, rc, d.R, d.base_fmt) > kSmemTwoPerSm) --stages;
+        if (k2_fp8_smem_bytes(r->tn, stages, rc, d.R, d.base_fmt) > kSmemTwoPerSm) stages = 12;
     }
     if (stages < 2 || stages > 12) return OB_ERR_TILE;
-    while (stages > 2 && k2_fp8_smem_bytes(r->tn, stages, rc, d.R, fp4 ? 1 : 0) > kSmemLimit) --stages;
-    if (k2_fp8_smem_bytes(r->tn, stages, rc, d.R, fp4 ? 1 : 0) > kSmemLimit) return OB_ERR_TILE;
-    if (fp4)   // TMEM: 2 tn accumulator columns + 32 scale-factor columns per ring slot, 512 in all
-        while (stages > 2 && 2 * r->tn + 32 * stages > 512) --stages;
+    while (stages > 2 && k2_fp8_smem_bytes(r->tn, stages, rc, d.R, d.base_fmt) > kSmemLimit) --stages;
+    if (k2_fp8_smem_bytes(r->tn, stages, rc, d.R, d.base_fmt) > kSmemLimit) return OB_ERR_TILE;
+    if (fp4)   // TMEM: 2 tn accumulator columns + 32 (MXFP4: 16) scale-factor columns per ring slot, 512 in all
+        while (stages > 2 && 2 * r->tn + sf_slot_bytes(d.base_fmt) / 64 * stages > 512) --stages;
     r->stages = stages;
     if ((long long)(d.L < r->tn ? d.L : r->tn) * (d.R / rc) > kMaxLoraIters) return OB_ERR_TOO_LARGE;
     r->wait_ms = (cfg && cfg->wait_ms > 0) ? (uint32_t)cfg->wait_ms : 2000u;
-    r->fused = (cfg && cfg->fused) ? 1 : 0;
+    r->fused = (cfg && cfg->fused && d.base_fmt != OB_BASE_MXFP4) ? 1 : 0;
     return OB_OK;
 }
 
@@ -424,8 +430,9 @@ int get_xmap(ObLayer* l, const void* xq, int rows, int tn, CUtensorMap* out) {
     m.rows = rows;
     m.tn = tn;
     const uint64_t lc = (uint64_t)(l->d.L < kMaxTileTenants ? l->d.L : kMaxTileTenants);
-    int st = tn == -4   // NVFP4 activation block scales as a [rows, 256] byte tensor: one 2 KB atom = an unswizzled 8-row box
-                 ? encode_2d(&m.tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, xq, 256, (uint64_t)rows, 256, 256, 8, true)
+    int st = tn == -4   // NVFP4, MXFP4 activation block scales as a [rows, 256] byte tensor: a K slot's = an unswizzled 8- or 4-row box
+                 ? encode_2d(&m.tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, xq, 256, (uint64_t)rows, 256, 256,
+                             (uint32_t)sf_slot_bytes(l->d.base_fmt) / 256, true)
              : tn == -2   // the shrink's per-tenant h blocks [S * rows, lc * R] bf16: boxes of a rank chunk x 128 rows
                  ? encode_2d(&m.tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, xq, lc * (uint64_t)l->d.R, (uint64_t)l->d.S * (uint64_t)rows,
                              lc * (uint64_t)l->d.R * 2, (uint32_t)l->rc, 128)
@@ -456,6 +463,8 @@ K1Params k1_params(ObLayer* l, const ObBatch* b, void* ws, const ObWorkspaceShap
     p.x = static_cast<const __nv_bfloat16*>(b->x);
     p.ldx = b->ldx;
     p.x_op = b->x_op;
+    p.x_codes = static_cast<const uint8_t*>(b->x_op == OB_X_QUANTIZED ? b->x_codes : nullptr);
+    p.x_scales = static_cast<const uint8_t*>(b->x_op == OB_X_QUANTIZED ? b->x_scales : nullptr);
     p.meta = meta_of(b);
     for (int s = 0; s < d.S; ++s) { p.a[s] = d.a[s]; p.sa[s] = d.sa[s]; }
     p.ag = d.ag;
@@ -464,7 +473,7 @@ K1Params k1_params(ObLayer* l, const ObBatch* b, void* ws, const ObWorkspaceShap
     p.hp = reinterpret_cast<float*>(base + lay.hp);
     p.max_m = sh->max_m;
     p.base_fmt = d.base_fmt;
-    p.tn = (r.big && d.base_fmt == OB_BASE_NVFP4) ? 256 : r.tn;   // the activation scales are laid out per token tile of K2
+    p.tn = (r.big && is_fp4(d)) ? 256 : r.tn;   // the activation scales are laid out per token tile of K2
     p.nblk = p.tn > 128 ? 2 : 1;
     p.kslots = (d.K + 255) / 256;
     p.rcp_approx = d.quant_rcp_approx;
@@ -518,7 +527,7 @@ int k1_fp8_impl(ObLayer* l, const ObBatch* b, void* ws, const ObWorkspaceShape* 
     if (r.big) {
         m.hcat = reinterpret_cast<__nv_bfloat16*>(base + lay.hcat);
         m.lc = d.L < kMaxTileTenants ? d.L : kMaxTileTenants;
-        const bool fp4 = d.base_fmt == OB_BASE_NVFP4;     // NVFP4: the output scale is alpha = 1 / (x_global * w_global) alone
+        const bool fp4 = is_fp4(d);                       // NVFP4, MXFP4: the output scale is alpha alone
         m.sx = fp4 ? nullptr : reinterpret_cast<const float*>(base + lay.sx);
         m.s_w = fp4 ? d.alpha : d.s_w;
     }
@@ -547,14 +556,14 @@ bool cluster_reduce_fits(const ObLayer* l, const Resolved& r, size_t smem) {
     static std::vector<std::pair<unsigned long long, int>> cache;   // (device, formats, split2, smem) -> resident clusters
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return false;
-    const int fp4 = l->d.base_fmt == OB_BASE_NVFP4 ? 1 : 0, stored = l->d.lora_fmt == kLoraBf16 ? 0 : 1;
-    const unsigned long long key = ((unsigned long long)dev << 48) | ((unsigned long long)(fp4 * 2 + stored) << 44) |
+    const int base = l->d.base_fmt, stored = l->d.lora_fmt == kLoraBf16 ? 0 : 1;
+    const unsigned long long key = ((unsigned long long)dev << 48) | ((unsigned long long)(base * 2 + stored) << 44) |
                                    ((unsigned long long)r.split2 << 40) | (unsigned long long)smem;
     std::lock_guard<std::mutex> g(mu);
     int n = -1;
     for (const auto& kv : cache) if (kv.first == key) n = kv.second;
     if (n < 0) {
-        n = k2_max_active_clusters(fp4, stored, r.split2, smem);
+        n = k2_max_active_clusters(base, stored, r.split2, smem);
         cache.emplace_back(key, n);
         if (std::getenv("LOWBIT_VERBOSE"))
             std::fprintf(stderr, "[onebase_b200] split-K clusters of %d CTAs, %zu B shared memory: %d resident at once\n", r.split2, smem, n);
@@ -568,7 +577,6 @@ struct K2Launch {
     CUtensorMap tm_x;
     dim3 grid;
     size_t smem;
-    bool fp4;
 };
 
 // `scratch` (optional): split-K partial tiles and arrival counters somewhere else than in the workspace's own split-K
@@ -637,8 +645,7 @@ int k2_prepare(ObLayer* l, const ObBatch* b, void* ws, const ObWorkspaceShape* s
     if (p.m_fast && l->n_tiles > 65535) return OB_ERR_TOO_LARGE;
     out->grid = p.m_fast ? dim3((unsigned)r.m_tiles, 1u, (unsigned)l->n_tiles)
                          : dim3((unsigned)l->n_tiles, (unsigned)r.split2, (unsigned)r.m_tiles);
-    out->fp4 = d.base_fmt == OB_BASE_NVFP4;
-    out->smem = k2_fp8_smem_bytes(r.tn, r.stages, l->rc, d.R, out->fp4 ? 1 : 0);
+    out->smem = k2_fp8_smem_bytes(r.tn, r.stages, l->rc, d.R, d.base_fmt);
     p.cluster_reduce = (scratch == nullptr && fused_ar == nullptr && cluster_reduce_fits(l, r, out->smem)) ? 1 : 0;
     if (fused_ar != nullptr) {      // the all-reduce of a row-parallel layer's output, inside the epilogue
         p.ar_world = fused_ar->world;
@@ -661,12 +668,12 @@ int k2_prefill_impl(ObLayer* l, const ObBatch* b, void* ws, const ObWorkspaceSha
     K2pParams p = {};
     p.M = b->M; p.N = d.N; p.K = d.K; p.S = d.S; p.R = d.R; p.L = d.L;
     for (int s = 0; s < OB_MAX_SLICES; ++s) p.widths[s] = s < d.S ? d.widths[s] : 0;
-    const bool fp4 = d.base_fmt == OB_BASE_NVFP4;
+    const bool fp4 = is_fp4(d);
     p.kblocks = (k_bytes(d) + kBlockK - 1) / kBlockK;
     p.lc = d.L < kMaxTileTenants ? d.L : kMaxTileTenants;
     p.max_m = sh->max_m;
     p.wait_ms = r.wait_ms;
-    p.s_w = fp4 ? d.alpha : d.s_w;               // NVFP4: one output scale, no per-token factor
+    p.s_w = fp4 ? d.alpha : d.s_w;               // NVFP4, MXFP4: one output scale, no per-token factor
     p.sx = fp4 ? nullptr : reinterpret_cast<const float*>(base + lay.sx);
     p.meta = meta_of(b);
     p.y = static_cast<__nv_bfloat16*>(b->y);
@@ -683,7 +690,7 @@ int k2_prefill_impl(ObLayer* l, const ObBatch* b, void* ws, const ObWorkspaceSha
         st = get_xmap(l, base + lay.xsf, (int)((lay.hp - lay.xsf) / 256), -4, &tm_sf[1]);
         if (st != OB_OK) return st;
     }
-    cudaError_t e = launch_k2_prefill_pair(p, l->tm_w, tm_x, tm_h, d.lora_fmt == kLoraBf16 ? l->tm_b : unused, tm_sf, r.pairs, fp4 ? 1 : 0, r.halves, pdl, stream);
+    cudaError_t e = launch_k2_prefill_pair(p, l->tm_w, tm_x, tm_h, d.lora_fmt == kLoraBf16 ? l->tm_b : unused, tm_sf, r.pairs, d.base_fmt, r.halves, pdl, stream);
     return e == cudaSuccess ? OB_OK : (int)e;
 }
 
@@ -701,8 +708,9 @@ int k2_stream_impl(ObLayer* l, const ObBatch* b, void* ws, const ObWorkspaceShap
     k.p.nh = k2_stream_h_tiles(r.tn);
     k.p.cluster_reduce = 0;
     k.p.m_fast = 0;
-    const size_t smem = k2_stream_smem_bytes(r.tn, r.stages, l->rc, l->d.R, l->d.S, k.fp4 ? 1 : 0);
-    cudaError_t e = launch_k2_stream(k.p, l->tm_w, k.tm_x, l->tm_b, r.grid_s, smem, k.fp4 ? 1 : 0, pdl, stream);
+    const int fp4 = is_fp4(l->d) ? 1 : 0;
+    const size_t smem = k2_stream_smem_bytes(r.tn, r.stages, l->rc, l->d.R, l->d.S, fp4);
+    cudaError_t e = launch_k2_stream(k.p, l->tm_w, k.tm_x, l->tm_b, r.grid_s, smem, fp4, pdl, stream);
     return e == cudaSuccess ? OB_OK : (int)e;
 }
 
@@ -713,8 +721,7 @@ int k2_fp8_impl(ObLayer* l, const ObBatch* b, void* ws, const ObWorkspaceShape* 
     K2Launch k;
     const int st = k2_prepare(l, b, ws, sh, r, chain, &k);
     if (st != OB_OK) return st;
-    cudaError_t e = k.fp4 ? launch_k2_nvfp4(k.p, l->tm_w, k.tm_x, l->tm_b, k.grid, k.smem, pdl, stream)
-                          : launch_k2_fp8(k.p, l->tm_w, k.tm_x, l->tm_b, k.grid, k.smem, pdl, stream);
+    cudaError_t e = launch_k2(l->d.base_fmt, k.p, l->tm_w, k.tm_x, l->tm_b, k.grid, k.smem, pdl, stream);
     return e == cudaSuccess ? OB_OK : (int)e;
 }
 
@@ -767,7 +774,7 @@ void resolve_big(const ObLayer* l, const ObBatch* b, Resolved* r) {
     // N = 8192 7 against 4 waves: 124 against 112.  (Whole calls over K = 1040, 3696, 4112, 7392 and 11280, six widths and nine
     // batches each: with 58 the choice takes 1.001 of the better side's time, at worst 1.07; with 55 1.002 and 1.10.)
     const long long w1 = (t1 + cap - 1) / cap, w2 = (t2 + cap - 1) / cap;
-    r->halves = d.base_fmt == OB_BASE_NVFP4 || w1 * (d.K % 128 == 0 ? 55 : 58) < w2 * 100 ? 1 : 2;
+    r->halves = is_fp4(d) || w1 * (d.K % 128 == 0 ? 55 : 58) < w2 * 100 ? 1 : 2;
     const long long tiles = r->halves == 1 ? t1 : t2;
     r->pairs = (int)(tiles < cap ? tiles : cap);
 }
@@ -869,7 +876,7 @@ int ob_k2_fp8_static(ObLayer* layer, const ObBatch* batch, void* workspace, cons
     if (st != OB_OK) return st;
     k.p.trace = nullptr;
     k.p.trace_ctas = 0;
-    cudaError_t e = launch_k2_fp8(k.p, layer->tm_w, k.tm_x, layer->tm_b, k.grid, k.smem, pdl, stream);
+    cudaError_t e = launch_k2(OB_BASE_FP8, k.p, layer->tm_w, k.tm_x, layer->tm_b, k.grid, k.smem, pdl, stream);
     return e == cudaSuccess ? OB_OK : (int)e;
 }
 
@@ -952,13 +959,15 @@ int ob_layer_create(const ObLayerDesc* desc, ObLayer** out) {
             }
         }
     }
-    // the large-tile prefill GEMM: slices in whole 16-byte pieces of y, NVFP4 base: whole 256-element k-blocks
+    // the large-tile prefill GEMM: slices in whole 16-byte pieces of y, NVFP4 and MXFP4 base: whole 256-element k-blocks
     l->big_ok = !b_sharded(*desc);
     for (int s = 0; s < desc->S; ++s) l->big_ok = l->big_ok && desc->widths[s] % 8 == 0;
-    if (desc->base_fmt == OB_BASE_NVFP4 && desc->K % 256 != 0) l->big_ok = false;
-    if (st == OB_OK && l->big_ok && desc->base_fmt == OB_BASE_NVFP4)
+    if (is_fp4(*desc) && desc->K % 256 != 0) l->big_ok = false;
+    if (st == OB_OK && l->big_ok && is_fp4(*desc)) {
+        const uint32_t slot_rows = (uint32_t)sf_slot_bytes(desc->base_fmt) / 256;
         st = encode_2d(&l->tm_wsf, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, desc->w_sf, 256,
-                       (uint64_t)l->n_tiles * (uint64_t)((desc->K + 255) / 256) * (kSfSlotBytes / 256), 256, 256, 8, true);
+                       (uint64_t)l->n_tiles * (uint64_t)((desc->K + 255) / 256) * slot_rows, 256, 256, slot_rows, true);
+    }
     if (st != OB_OK) {
         delete l;
         return st;
@@ -1047,6 +1056,53 @@ int ob_chain_nvfp4(ObLayer* layer, const ObBatch* batch, void* workspace, const 
     return k2_fp8_impl(layer, batch, workspace, shape, r, 1, stream, r.stream != 0);
 }
 
+int ob_k1_mxfp4(ObLayer* layer, const ObBatch* batch, void* workspace, const ObWorkspaceShape* shape, const ObTileCfg* cfg,
+                void* cuda_stream) {
+    Resolved r;
+    int st = prepare_call(layer, batch, workspace, shape, cfg, &r, OB_BASE_MXFP4);
+    if (st != OB_OK) return st;
+    return k1_fp8_impl(layer, batch, workspace, shape, r, 0, static_cast<cudaStream_t>(cuda_stream), false, true);
+}
+
+int ob_k2_mxfp4(ObLayer* layer, const ObBatch* batch, void* workspace, const ObWorkspaceShape* shape, const ObTileCfg* cfg,
+                int pdl, void* cuda_stream) {
+    Resolved r;
+    int st = prepare_call(layer, batch, workspace, shape, cfg, &r, OB_BASE_MXFP4);
+    if (st != OB_OK) return st;
+    return k2_fp8_impl(layer, batch, workspace, shape, r, pdl, static_cast<cudaStream_t>(cuda_stream));
+}
+
+int ob_chain_mxfp4(ObLayer* layer, const ObBatch* batch, void* workspace, const ObWorkspaceShape* shape, const ObTileCfg* cfg,
+                   void* cuda_stream) {
+    Resolved r;
+    int st = prepare_call(layer, batch, workspace, shape, cfg, &r, OB_BASE_MXFP4);
+    if (st != OB_OK) return st;
+    cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+    st = k1_fp8_impl(layer, batch, workspace, shape, r, 1, stream);
+    if (st != OB_OK) return st;
+    return k2_fp8_impl(layer, batch, workspace, shape, r, 1, stream);
+}
+
+int ob_mxfp4_packed_scale_bytes(int32_t K, int32_t S, const int32_t* widths, size_t* bytes) {
+    size_t nv = 0;
+    const int st = ob_nvfp4_packed_scale_bytes(K, S, widths, bytes ? &nv : nullptr);   // the same slots, twice the bytes
+    if (st != OB_OK) return st;
+    *bytes = nv / 2;
+    return OB_OK;
+}
+
+int ob_mxfp4_pack_scales(const void* w_sf_linear, int32_t K, int32_t S, const int32_t* widths, void* packed,
+                         size_t packed_bytes, void* cuda_stream) {
+    size_t need = 0;
+    int st = ob_mxfp4_packed_scale_bytes(K, S, widths, &need);
+    if (st != OB_OK) return st;
+    if (!w_sf_linear || !packed) return OB_ERR_NULL;
+    if (packed_bytes < need) return OB_ERR_WORKSPACE;
+    cudaError_t e = launch_pack_scales(OB_BASE_MXFP4, static_cast<const uint8_t*>(w_sf_linear), K, S, widths, static_cast<uint8_t*>(packed),
+                                       need, static_cast<cudaStream_t>(cuda_stream));
+    return e == cudaSuccess ? OB_OK : (int)e;
+}
+
 int ob_nvfp4_packed_scale_bytes(int32_t K, int32_t S, const int32_t* widths, size_t* bytes) {
     if (!widths || !bytes) return OB_ERR_NULL;
     if (K < 32 || K % 32 != 0 || S < 1 || S > OB_MAX_SLICES) return OB_ERR_SHAPE;
@@ -1066,7 +1122,7 @@ int ob_nvfp4_pack_scales(const void* w_sf_linear, int32_t K, int32_t S, const in
     if (st != OB_OK) return st;
     if (!w_sf_linear || !packed) return OB_ERR_NULL;
     if (packed_bytes < need) return OB_ERR_WORKSPACE;
-    cudaError_t e = launch_pack_scales(static_cast<const uint8_t*>(w_sf_linear), K, S, widths, static_cast<uint8_t*>(packed),
+    cudaError_t e = launch_pack_scales(OB_BASE_NVFP4, static_cast<const uint8_t*>(w_sf_linear), K, S, widths, static_cast<uint8_t*>(packed),
                                        need, static_cast<cudaStream_t>(cuda_stream));
     return e == cudaSuccess ? OB_OK : (int)e;
 }
@@ -1238,8 +1294,7 @@ int ob_chain_allreduce(ObLayer* layer, const ObBatch* batch, void* workspace, co
     K2Launch k;
     st = k2_prepare(layer, batch, workspace, shape, r, false, &k, nullptr, comm);
     if (st != OB_OK) return st;
-    cudaError_t e = k.fp4 ? launch_k2_nvfp4(k.p, layer->tm_w, k.tm_x, layer->tm_b, k.grid, k.smem, 1, stream)
-                          : launch_k2_fp8(k.p, layer->tm_w, k.tm_x, layer->tm_b, k.grid, k.smem, 1, stream);
+    cudaError_t e = launch_k2(layer->d.base_fmt, k.p, layer->tm_w, k.tm_x, layer->tm_b, k.grid, k.smem, 1, stream);
     return e == cudaSuccess ? OB_OK : (int)e;
 }
 

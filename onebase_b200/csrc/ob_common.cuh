@@ -28,11 +28,16 @@ constexpr int kMmaShrinkTokensStored = 1024;
 constexpr int kDecodeTokens = 32;     // batches up to this size take the decode forms (one position per shrink warp)
 constexpr int kCounterSlots = 4096;  // split-K arrival counters in the workspace
 constexpr int kStreamMaxCtas = 256;  // most CTAs of the persistent decode GEMM (one per SM)
-constexpr int kSfSlotBytes = 2048;
+constexpr int kSfSlotBytes = 2048;   // NVFP4: scale factors of 128 rows x one 256-element K slot (4 atoms of 512 bytes)
+// Scale factors of 128 rows x one 256-element K slot by base format: 16 per row (NVFP4) or 8 (MXFP4), in atoms of 512 bytes
+// (128 rows x 4 scales).  The workspace and the packed weights of either are laid out in slots of this size.
+__host__ __device__ constexpr int sf_slot_bytes(int base_fmt) {
+    return base_fmt == OB_BASE_NVFP4 ? kSfSlotBytes : base_fmt == OB_BASE_MXFP4 ? kSfSlotBytes / 2 : 0;
+}
 // Peer-memory all-reduce: layout of a rank's communication buffer (see allreduce.cu)
 constexpr int kArStateBytes = 16384;  // state words, rank flags, per-tile flags; the staged copies follow
 constexpr int kArFlagsOff = 1024, kArFlags2Off = 2048, kArTileFlagsOff = 4096;
-constexpr int kArMaxTiles = 384;      // per-tile flags [world][kArMaxTiles] of the all-reduce fused into K2's epilogue   // NVFP4: scale factors of 128 rows x one 256-element K slot (4 atoms of 512 bytes)
+constexpr int kArMaxTiles = 384;      // per-tile flags [world][kArMaxTiles] of the all-reduce fused into K2's epilogue
 
 __host__ __device__ inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
@@ -42,7 +47,7 @@ struct WorkspaceLayout {
     size_t counters;   // int32 [kCounterSlots]   zero between launches
     size_t sx;         // fp32  [max_m]           per-position activation scale
     size_t xq;         // bytes [max_m * max_k]   quantized activations, row pitch = the calling layer's K (FP8) or K/2
-    size_t xsf;        // bytes NVFP4 activation block scales: [token tile][256-element K slot][128-token block][2048]
+    size_t xsf;        // bytes NVFP4 activation block scales: [token tile][256-element K slot][128-token block][2048] (MXFP4: [1024])
     size_t hp;         // fp32  [max_split1 * max_sr * max_m]  shrink partials [split][slice][position][rank]
     size_t part;       // fp32  [max_split2 * token tile * (max_n rounded to tiles)]  GEMM split-K partials
     size_t xs;         // bf16  [max_m * max_k]   adapter-sorted copy of x for the tensor-core shrink (max_m > 32 only)
@@ -100,6 +105,8 @@ struct K1Params {
     const __nv_bfloat16* x;
     int64_t ldx;
     int x_op;              // OB_X_SILU_MUL: x is [M, 2K] (gate | up) and the projection's input is bf16(bf16(silu(g)) * u)
+    const uint8_t* x_codes;   // OB_X_QUANTIZED: x's codes and scales as the caller made them (dense rows of x, not positions)
+    const uint8_t* x_scales;
     Meta meta;
     const void* a[OB_MAX_SLICES];
     const void* sa[OB_MAX_SLICES];
@@ -108,11 +115,12 @@ struct K1Params {
     float* sx;             // [M]
     float* hp;             // [split1][S][max_m][R]
     int max_m;
-    int base_fmt;          // OB_BASE_FP8: per-token e4m3 quantization; OB_BASE_NVFP4: e2m1 codes + ue4m3 scale per 16
-    int tn, nblk, kslots;  // NVFP4: K2's token tile, its 128-token scale blocks, 256-element K slots (scale layout)
+    int base_fmt;          // OB_BASE_FP8: per-token e4m3 quantization; OB_BASE_NVFP4: e2m1 codes + ue4m3 scale per 16; OB_BASE_MXFP4:
+                           // e2m1 codes + power-of-two scale per 32
+    int tn, nblk, kslots;  // NVFP4, MXFP4: K2's token tile, its 128-token scale blocks, 256-element K slots (scale layout)
     int rcp_approx;        // NVFP4: 1 = rcp.approx.ftz reciprocals (vLLM's CUDA quantizer), 0 = IEEE (the torch recipe)
     const float* x_global; // NVFP4: [1] static activation global scale
-    uint8_t* xsf;          // NVFP4: activation block scales, packed per (token tile, K slot) in scale-factor atoms
+    uint8_t* xsf;          // NVFP4, MXFP4: activation block scales, packed per (token tile, K slot) in scale-factor atoms
     __nv_bfloat16* xs;     // prefill with a tensor-core shrink: the quantizing CTAs also copy their row here (null: no copy)
     int32_t* xq_ready;     // chain: counts the positions whose codes and scale are written (null: no signal)
     unsigned long long* trace;   // optional timeline buffer (null: off); K1 stamps go after K2's region
@@ -207,10 +215,10 @@ struct K2Params {
     int b_row0[OB_MAX_SLICES];   // first output feature of each slice whose B rows this rank holds (0 unless B is sharded)
     int b_rows[OB_MAX_SLICES];   // number of those rows (the slice's width unless B is sharded)
     const float* bg;
-    const uint8_t* wsf;    // NVFP4 base: W block scales, packed per (128-row tile, 256-element K slot) in scale-factor atoms
-    const uint8_t* xsf;    // NVFP4 base: K1's activation block scales, packed per (token tile, K slot)
-    const float* alpha;    // NVFP4 base: [1] 1 / (x_global * w_global)
-    int nblk;              // NVFP4 base: 128-token scale-factor blocks per token tile (1, or 2 for 256-token tiles)
+    const uint8_t* wsf;    // NVFP4, MXFP4 base: W block scales, packed per (128-row tile, 256-element K slot) in scale-factor atoms
+    const uint8_t* xsf;    // NVFP4, MXFP4 base: K1's activation block scales, packed per (token tile, K slot)
+    const float* alpha;    // NVFP4 base: [1] 1 / (x_global * w_global); MXFP4 base: [1] the base product's factor
+    int nblk;              // NVFP4, MXFP4 base: 128-token scale-factor blocks per token tile (1, or 2 for 256-token tiles)
     int32_t* xq_ready;     // chain: K1's count of quantized positions; the producer polls it instead of waiting for all of K1
     int32_t* chain_done;   // chain: CTAs of this launch that finished; the last one clears the chain's words
     int32_t* work_quant;   // fused: next position to quantize (claimed by a CTA's four epilogue warps together)

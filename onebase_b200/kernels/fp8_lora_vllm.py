@@ -205,7 +205,12 @@ class VllmFusedFP8LoRA:
         return self.scratch.region("hp", 4 * n).view(torch.float32).view(split1, self.S, max_m, self.R)
 
     # ------------------------------------------------------------------------------------------------- the call
-    def _batch(self, x, meta_args, out, silu_mul: bool = False, residual=None):
+    def _codes_ok(self, codes, scales, M: int) -> bool:
+        """Whether `quantized=` fits: e4m3 codes [M, K] and fp32 scales [M], as rms_norm(quant="fp8") gives them."""
+        return (codes.dtype == torch.float8_e4m3fn and tuple(codes.shape) == (M, self.K) and scales.dtype == torch.float32 and
+                tuple(scales.shape) == (M,))
+
+    def _batch(self, x, meta_args, out, silu_mul: bool = False, residual=None, quantized=None):
         tok, srt, seg_n, seg_start, seg_ids = meta_args[:5]
         M = x.shape[0]
         assert x.dtype == torch.bfloat16 and x.dim() == 2 and x.stride(1) == 1
@@ -220,16 +225,26 @@ class VllmFusedFP8LoRA:
         if residual is not None:
             assert residual.dtype == torch.bfloat16 and residual.shape == (M, self.N) and residual.stride(1) == 1
             b.residual, b.ldr = residual.data_ptr(), residual.stride(0)
+        if quantized is not None:
+            codes, scales = quantized
+            if silu_mul:
+                raise ValueError("quantized= and silu_mul= exclude one another: the codes are those of the projection's input")
+            if not self._codes_ok(codes, scales, M) or not (codes.is_contiguous() and scales.is_contiguous()) or \
+                    codes.device != x.device or scales.device != x.device:
+                raise ValueError(f"quantized= must be dense (codes, scales) of x [{M}, {self.K}] in the base's format, on x's device")
+            b.x_op, b.x_codes, b.x_scales = _lib.OB_X_QUANTIZED, codes.data_ptr(), scales.data_ptr()
         return b, y
 
     def __call__(self, x, meta_args, out=None, cfg: dict | None = None, pdl: bool = True, shrink: bool = True,
-                 gemm: bool = True, allreduce=None, silu_mul: bool = False, residual=None):
+                 gemm: bool = True, allreduce=None, silu_mul: bool = False, residual=None, quantized=None):
         """y = x W^T (FP8, x quantized per token as vLLM does) + every tenant's expansion.  pdl=False runs the same two
         kernels serialized; shrink=False / gemm=False run one kernel alone (breakdowns and tests).  allreduce = a
         tp.PeerComm: this is a row-parallel shard and y is summed over the ranks inside K2's epilogue (ob_chain_allreduce).
         silu_mul=True: x is the merged gate | up output [M, 2K] and the projection's input is silu(gate) * up, formed inside
-        K1 (down_proj).  residual = [M, N] bf16: K2 stores y + residual, the new residual stream (o_proj, down_proj)."""
-        b, y = self._batch(x, meta_args, out, silu_mul, residual)
+        K1 (down_proj).  residual = [M, N] bf16: K2 stores y + residual, the new residual stream (o_proj, down_proj).
+        quantized = (codes, scales): x's codes in the base's format (rms_norm's, mxfp4.quantize's), which K1 takes instead of
+        quantizing x; x itself is what the adapters multiply."""
+        b, y = self._batch(x, meta_args, out, silu_mul, residual, quantized)
         t = self.tile(b.M, cfg)
         ws, sh = C.c_void_p(self.scratch.ptr), C.byref(self.scratch.shape)
         st = C.c_void_p(torch.cuda.current_stream(x.device).cuda_stream)

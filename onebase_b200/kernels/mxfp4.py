@@ -2,7 +2,7 @@
 libonebase_b200.so: quantization of weights and activations, and the values codes stand for.
 
 codes [..., K/2] uint8 hold two elements per byte (element 2i in the low nibble), scales [..., K/32] uint8 exponent + 127 (255:
-NaN)."""
+NaN) -- what VllmFusedMXFP4LoRA takes as its weight, and as its input under `quantized=`."""
 from __future__ import annotations
 
 import ctypes as C

@@ -89,6 +89,9 @@ class VllmFusedNVFP4LoRA(VllmFusedFP8LoRA):
             _lib.call("ob_layer_create", C.byref(d), C.byref(h))
         self._h = h
 
+    def _codes_ok(self, codes, scales, M: int) -> bool:
+        return False                                # nothing here makes NVFP4 activations but the projection itself
+
     def set_x_global(self, x_global: float) -> None:
         """Refill the static activation scale and alpha on the device (reference: op.x_global.fill_ / op.alpha.fill_)."""
         self.x_global.fill_(float(x_global))

@@ -1,7 +1,13 @@
 """Root-mean-square norm with the residual's addition before it and low-precision codes behind it, on B200 through
 libonebase_b200.so (ob_rms_norm).
 
-In a decoder layer it stands in front of qkv_proj and gate_up_proj, and, on [tokens, heads, head size], it is the norm of queries and keys.  The reference leaves the norm to vLLM (RMSNorm,
+In a decoder layer it stands in front of qkv_proj and gate_up_proj and gives a fused projection its input together with the
+codes the projection multiplies:
+
+    n = rms_norm(x, weight, eps, residual=stream, quant="fp8")
+    y = op(n.y, meta, quantized=(n.codes, n.scales))        # VllmFusedFP8LoRA; quant="mxfp4" for VllmFusedMXFP4LoRA
+
+and, on [tokens, heads, head size], it is the norm of queries and keys.  The reference leaves the norm to vLLM (RMSNorm,
 vllm/model_executor/layers/layernorm.py).
 """
 from __future__ import annotations

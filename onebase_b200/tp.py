@@ -85,6 +85,26 @@ def shard_row_nvfp4(w_q4, w_sf, a_stacked, b_stacked, tp: int, rank: int):
             tuple(a[..., lo:lo + ks].contiguous() for a in a_stacked), tuple(b_stacked))
 
 
+def shard_column_mxfp4(w_q, w_sf, a_stacked, b_stacked, tp: int, rank: int, replicate=()):
+    """Column-parallel shard of an MXFP4 base: the rank's rows of the packed codes [N, K/2] and of the scale bytes [N, K/32].
+    Returns (w_q, w_sf, a_stacked, b_stacked)."""
+    q_r, a_r, b_r = shard_column(w_q, a_stacked, b_stacked, tp, rank, replicate)
+    sf_r, _, _ = shard_column(w_sf, a_stacked, b_stacked, tp, rank, replicate)
+    return q_r, sf_r, a_r, b_r
+
+
+def shard_row_mxfp4(w_q, w_sf, a_stacked, b_stacked, tp: int, rank: int):
+    """Row-parallel shard of an MXFP4 base: columns [lo/2, hi/2) of the codes and [lo/32, hi/32) of the scale bytes (K/tp a multiple of
+    32: whole blocks).  Quantization is block-local, so a rank's codes of its K slice equal the unsharded ones.  Returns (w_q, w_sf,
+    a_stacked, b_stacked)."""
+    K = w_q.shape[1] * 2
+    assert K % tp == 0 and (K // tp) % 32 == 0, f"K = {K} does not split into {tp} shards of whole 32-element blocks"
+    ks = K // tp
+    lo = rank * ks
+    return (w_q[:, lo // 2:(lo + ks) // 2].contiguous(), w_sf[:, lo // 32:(lo + ks) // 32].contiguous(),
+            tuple(a[..., lo:lo + ks].contiguous() for a in a_stacked), tuple(b_stacked))
+
+
 def run_row_parallel_sharded(op, x_r, meta_args, out=None, cfg=None, group=None):
     """One row-parallel projection with sharded adapters on this rank: K1 on the rank's K slice, all-reduce of the fp32
     shrink partials (a few hundred KB at most), K2 with the expand on the rank's output features only, all-reduce of y.

@@ -71,3 +71,9 @@ def zipf_request_ids(M: int, L: int, seed: int, alpha: float = 1.1, mean_len: in
         ids[pos:pos + n] = slot
         pos += n
     return ids
+
+
+def with_mxfp4_base(d: dict) -> dict:
+    from oracle import mxfp4
+    d["w_mx"], d["w_mx_sf"] = mxfp4.quant(d["w"].to(torch.bfloat16))
+    return d

@@ -160,8 +160,9 @@ def _meta(ids, L):
     return tuple(t.to(DEV) for t in (ids, torch.argsort(ids, stable=True).to(torch.int32), seg_n, seg_start, seg_ids))
 
 
-def _graphed(call, keep):
-    """`call` captured in a CUDA graph: a function that replays it and gives the outputs of the capture."""
+def _graphed(call):
+    """`call` captured in a CUDA graph: a function that replays it and gives the outputs of the capture.  It keeps `call`, and
+    with it the projection whose weights the graph reads."""
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -175,7 +176,7 @@ def _graphed(call, keep):
         graph.replay()
         return out
 
-    replay.keep = (graph, keep)
+    replay.keep = call
     return replay
 
 
@@ -209,7 +210,7 @@ def prepare(case, seed):
     if own:
         s["call"] = _own_call(s)
         if case.get("tokens", MAX_M) * case.get("heads", 1) <= GRAPH_M:
-            s["call"] = _graphed(s["call"], s)
+            s["call"] = _graphed(s["call"])
     return s
 
 

@@ -36,22 +36,34 @@ __device__ __forceinline__ void mx_load8(const T* src, float (&v)[8]) {
     }
 }
 
-template <typename T, bool VEC>
+// Where group i of eight elements lies: dense tensors are one long row (no division); else row i / vpr, in 32 bits while they suffice.
+template <bool DENSE>
+__device__ __forceinline__ long long mx_offset(long long i, long long total, int vpr, long long ld) {
+    if (DENSE) return i * 8;
+    const long long row = total <= 0xFFFFFFFFll ? (long long)((uint32_t)i / (uint32_t)vpr) : i / vpr;
+    return row * ld + (i - row * vpr) * 8;
+}
+
+template <typename T, bool VEC, bool DENSE, int U>
 __global__ void __launch_bounds__(kMxThreads)
-mxfp4_quantize_kernel(const T* __restrict__ x, long long rows, int K, long long ldx, uint32_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+mxfp4_quantize_kernel(const T* __restrict__ x, long long total, int vpr, long long ldx, uint32_t* __restrict__ codes, uint8_t* __restrict__ scales) {
     griddep_launch_dependents();
     griddep_wait();
-    const int vpr = K >> 3;                           // groups of eight per row, a multiple of four
-    const long long total = rows * vpr;
-    for (long long g = (long long)blockIdx.x * kMxThreads; g < total; g += (long long)gridDim.x * kMxThreads) {
-        const long long i = g + threadIdx.x;          // (the four lanes of a block are all in range, or none is)
-        float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        if (i < total) {
-            const long long row = i / vpr;
-            mx_load8<T, VEC>(x + row * ldx + (i - row * vpr) * 8, v);
-        }
+    const long long i0 = (long long)blockIdx.x * (kMxThreads * U) + threadIdx.x;
+    float v[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {                     // (the four lanes of a block are all in range, or none is)
+        const long long i = i0 + u * kMxThreads;
+        if (i < total) mx_load8<T, VEC>(x + mx_offset<DENSE>(i, total, vpr, ldx), v[u]);
+        else
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[u][e] = 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const long long i = i0 + u * kMxThreads;
         uint32_t byte;
-        const uint32_t c = mx_quantize8(v, byte);
+        const uint32_t c = mx_quantize8(v[u], byte);
         if (i < total) {
             codes[i] = c;
             if ((i & 3) == 0) scales[i >> 2] = (uint8_t)byte;
@@ -83,58 +95,86 @@ __device__ __forceinline__ void mx_store8(T* dst, const float (&v)[8]) {
     }
 }
 
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool DENSE, int U>
 __global__ void __launch_bounds__(kMxThreads)
-mxfp4_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales, long long rows, int K, T* __restrict__ out, long long ldo) {
+mxfp4_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales, long long total, int vpr, T* __restrict__ out, long long ldo) {
     griddep_launch_dependents();
     griddep_wait();
-    const int vpr = K >> 3;
-    const long long total = rows * vpr;
-    for (long long i = (long long)blockIdx.x * kMxThreads + threadIdx.x; i < total; i += (long long)gridDim.x * kMxThreads) {
+    const long long i0 = (long long)blockIdx.x * (kMxThreads * U) + threadIdx.x;
+    uint32_t c[U], byte[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const long long i = i0 + u * kMxThreads;
+        c[u] = i < total ? __ldg(codes + i) : 0u;
+        byte[u] = i < total ? __ldg(scales + (i >> 2)) : 0u;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const long long i = i0 + u * kMxThreads;
         float v[8];
-        e2m1x8_values(codes[i], v);
-        const float sc = mx_scale(scales[i >> 2]);
+        e2m1x8_values(c[u], v);
+        const float sc = mx_scale(byte[u]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] *= sc;
-        const long long row = i / vpr;
-        mx_store8<T, VEC>(out + row * ldo + (i - row * vpr) * 8, v);
+        if (i < total) mx_store8<T, VEC>(out + mx_offset<DENSE>(i, total, vpr, ldo), v);
     }
 }
 
-static cudaLaunchConfig_t mx_config(long long total, cudaStream_t stream, cudaLaunchAttribute* attr) {
+template <typename... Params, typename... Args>
+static cudaError_t mx_launch(void (*kernel)(Params...), long long total, int unroll, cudaStream_t stream, Args... args) {
     cudaLaunchConfig_t cfg = {};
-    long long blocks = (total + kMxThreads - 1) / kMxThreads;
-    if (blocks > (1 << 30)) blocks = 1 << 30;
-    cfg.gridDim = dim3((unsigned)blocks);
+    const long long per = (long long)kMxThreads * unroll, ctas = (total + per - 1) / per;
+    if (ctas > 0x7fffffffll) return cudaErrorInvalidValue;
+    cfg.gridDim = dim3((unsigned)ctas);
     cfg.blockDim = dim3(kMxThreads);
     cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cfg;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// Tensors that fill the GPU take four groups per thread (their loads in flight together), smaller ones one.
+static bool mx_large(long long total) { return total > 148LL * 2048 * 4; }
+
+template <typename T, bool VEC, bool DENSE>
+static cudaError_t quantize_form(const T* x, long long total, int vpr, long long ldx, uint32_t* codes, uint8_t* scales, cudaStream_t stream) {
+    return mx_large(total) ? mx_launch(mxfp4_quantize_kernel<T, VEC, DENSE, 4>, total, 4, stream, x, total, vpr, ldx, codes, scales)
+                           : mx_launch(mxfp4_quantize_kernel<T, VEC, DENSE, 1>, total, 1, stream, x, total, vpr, ldx, codes, scales);
 }
 
 template <typename T>
-static cudaError_t quantize_typed(const void* x, long long rows, int K, long long ldx, void* codes, void* scales, cudaStream_t stream) {
-    cudaLaunchAttribute attr[1];
-    const cudaLaunchConfig_t cfg = mx_config(rows * (K >> 3), stream, attr);
-    const bool vec = (reinterpret_cast<uintptr_t>(x) & 15u) == 0 && (ldx * (long long)sizeof(T)) % 16 == 0;
-    return vec ? cudaLaunchKernelEx(&cfg, mxfp4_quantize_kernel<T, true>, static_cast<const T*>(x), rows, K, ldx, static_cast<uint32_t*>(codes),
-                                    static_cast<uint8_t*>(scales))
-               : cudaLaunchKernelEx(&cfg, mxfp4_quantize_kernel<T, false>, static_cast<const T*>(x), rows, K, ldx, static_cast<uint32_t*>(codes),
-                                    static_cast<uint8_t*>(scales));
+static cudaError_t quantize_typed(const void* xp, long long rows, int K, long long ldx, void* codes, void* scales, cudaStream_t stream) {
+    const T* x = static_cast<const T*>(xp);
+    uint32_t* c = static_cast<uint32_t*>(codes);
+    uint8_t* s = static_cast<uint8_t*>(scales);
+    const int vpr = K >> 3;
+    const long long total = rows * vpr;
+    if ((reinterpret_cast<uintptr_t>(xp) & 15u) != 0 || (rows > 1 && (ldx * (long long)sizeof(T)) % 16 != 0))
+        return quantize_form<T, false, false>(x, total, vpr, ldx, c, s, stream);
+    return rows == 1 || ldx == K ? quantize_form<T, true, true>(x, total, vpr, ldx, c, s, stream)
+                                 : quantize_form<T, true, false>(x, total, vpr, ldx, c, s, stream);
+}
+
+template <typename T, bool VEC, bool DENSE>
+static cudaError_t dequantize_form(const uint32_t* codes, const uint8_t* scales, long long total, int vpr, T* out, long long ldo, cudaStream_t stream) {
+    return mx_large(total) ? mx_launch(mxfp4_dequantize_kernel<T, VEC, DENSE, 4>, total, 4, stream, codes, scales, total, vpr, out, ldo)
+                           : mx_launch(mxfp4_dequantize_kernel<T, VEC, DENSE, 1>, total, 1, stream, codes, scales, total, vpr, out, ldo);
 }
 
 template <typename T>
-static cudaError_t dequantize_typed(const void* codes, const void* scales, long long rows, int K, void* out, long long ldo, cudaStream_t stream) {
-    cudaLaunchAttribute attr[1];
-    const cudaLaunchConfig_t cfg = mx_config(rows * (K >> 3), stream, attr);
-    const bool vec = (reinterpret_cast<uintptr_t>(out) & 15u) == 0 && (ldo * (long long)sizeof(T)) % 16 == 0;
-    return vec ? cudaLaunchKernelEx(&cfg, mxfp4_dequantize_kernel<T, true>, static_cast<const uint32_t*>(codes), static_cast<const uint8_t*>(scales),
-                                    rows, K, static_cast<T*>(out), ldo)
-               : cudaLaunchKernelEx(&cfg, mxfp4_dequantize_kernel<T, false>, static_cast<const uint32_t*>(codes), static_cast<const uint8_t*>(scales),
-                                    rows, K, static_cast<T*>(out), ldo);
+static cudaError_t dequantize_typed(const void* codes, const void* scales, long long rows, int K, void* outp, long long ldo, cudaStream_t stream) {
+    const uint32_t* c = static_cast<const uint32_t*>(codes);
+    const uint8_t* s = static_cast<const uint8_t*>(scales);
+    T* out = static_cast<T*>(outp);
+    const int vpr = K >> 3;
+    const long long total = rows * vpr;
+    if ((reinterpret_cast<uintptr_t>(outp) & 15u) != 0 || (rows > 1 && (ldo * (long long)sizeof(T)) % 16 != 0))
+        return dequantize_form<T, false, false>(c, s, total, vpr, out, ldo, stream);
+    return rows == 1 || ldo == K ? dequantize_form<T, true, true>(c, s, total, vpr, out, ldo, stream)
+                                 : dequantize_form<T, true, false>(c, s, total, vpr, out, ldo, stream);
 }
 
 cudaError_t launch_mxfp4_quantize(const void* x, int dtype, long long rows, int K, long long ldx, void* codes, void* scales, cudaStream_t stream) {

@@ -261,8 +261,7 @@ int ob_chain_nvfp4(ObLayer* layer, const ObBatch* batch, void* workspace, const 
                    const ObTileCfg* cfg, void* cuda_stream);
 
 /* The MXFP4-base counterparts: K1 quantizes x to e2m1 codes with a power-of-two scale per 32 elements (ob_mxfp4_quantize's rule) and
- * shrinks; K2 is the block-scaled tcgen05 GEMM (kind::mxf4), y = alpha sum v(x) v(w) + LoRA, K a multiple of 32 (the large prefill tiles: of
- * 256).  The persistent and the one-kernel decode forms (ObTileCfg.stream, .fused) do not exist for this base: asked for, the call takes
+ * shrinks; K2 is the block-scaled tcgen05 GEMM (kind::mxf4), y = alpha sum v(x) v(w) + LoRA, K a multiple of 32.  The persistent and the one-kernel decode forms (ObTileCfg.stream, .fused) do not exist for this base: asked for, the call takes
  * the two-kernel chain.  No counterpart in the reference (its 4-bit base is NVFP4). */
 int ob_k1_mxfp4(ObLayer* layer, const ObBatch* batch, void* workspace, const ObWorkspaceShape* shape, const ObTileCfg* cfg, void* cuda_stream);
 int ob_k2_mxfp4(ObLayer* layer, const ObBatch* batch, void* workspace, const ObWorkspaceShape* shape, const ObTileCfg* cfg, int pdl,

@@ -9,6 +9,8 @@ import ctypes as C
 import os
 from pathlib import Path
 
+import torch
+
 PKG = Path(__file__).resolve().parent
 LIB_PATH = PKG / "lib" / "libonebase_b200.so"
 
@@ -159,3 +161,11 @@ def check(fn: str, status: int) -> None:
 
 def call(fn: str, *args) -> None:
     check(fn, getattr(lib(), fn)(*args))
+
+
+def call_on(device, fn: str, *args) -> None:
+    """`fn(*args, stream)` on `device` (a torch CUDA device) and its current stream."""
+    if device.index is not None and device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return call(fn, *args, torch.cuda.current_stream().cuda_stream)
+    call(fn, *args, torch.cuda.current_stream().cuda_stream)

@@ -959,10 +959,11 @@ int ob_layer_create(const ObLayerDesc* desc, ObLayer** out) {
             }
         }
     }
-    // the large-tile prefill GEMM: slices in whole 16-byte pieces of y, NVFP4 and MXFP4 base: whole 256-element k-blocks
+    // the large-tile prefill GEMM: slices in whole 16-byte pieces of y; NVFP4 base: whole 256-element k-blocks (the MXFP4 base's last one
+    // may be ragged: codes past K arrive as zeros, both sides' scales as the byte 0)
     l->big_ok = !b_sharded(*desc);
     for (int s = 0; s < desc->S; ++s) l->big_ok = l->big_ok && desc->widths[s] % 8 == 0;
-    if (is_fp4(*desc) && desc->K % 256 != 0) l->big_ok = false;
+    if (desc->base_fmt == OB_BASE_NVFP4 && desc->K % 256 != 0) l->big_ok = false;
     if (st == OB_OK && l->big_ok && is_fp4(*desc)) {
         const uint32_t slot_rows = (uint32_t)sf_slot_bytes(desc->base_fmt) / 256;
         st = encode_2d(&l->tm_wsf, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, desc->w_sf, 256,

@@ -26,9 +26,7 @@ def pack_weight_scales(w_sf: torch.Tensor, K: int, widths) -> torch.Tensor:
     n = C.c_size_t()
     _lib.call("ob_mxfp4_packed_scale_bytes", K, len(widths), wa, C.byref(n))
     out = torch.empty(n.value, dtype=torch.uint8, device=w_sf.device)
-    with torch.cuda.device(w_sf.device):
-        _lib.call("ob_mxfp4_pack_scales", C.c_void_p(w_sf.data_ptr()), K, len(widths), wa, C.c_void_p(out.data_ptr()), n.value,
-                  C.c_void_p(torch.cuda.current_stream(w_sf.device).cuda_stream))
+    _lib.call_on(w_sf.device, "ob_mxfp4_pack_scales", w_sf.data_ptr(), K, len(widths), wa, out.data_ptr(), n.value)
     return out
 
 

@@ -85,6 +85,5 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 1e-6,
         n.y, (n.y_ld, n.y_hd) = y.data_ptr(), _strides(y)
     if codes is not None:
         n.codes, n.scales = codes.data_ptr(), scales.data_ptr()
-    with torch.cuda.device(x.device):
-        _lib.call("ob_rms_norm", C.byref(n), C.c_void_p(torch.cuda.current_stream(x.device).cuda_stream))
+    _lib.call_on(x.device, "ob_rms_norm", C.byref(n))
     return NormOut(y, residual_out, codes, scales)

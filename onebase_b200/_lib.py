@@ -163,9 +163,14 @@ def call(fn: str, *args) -> None:
     check(fn, getattr(lib(), fn)(*args))
 
 
+# (the handle alone: building a torch Stream object costs a call more than its launch)
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def call_on(device, fn: str, *args) -> None:
     """`fn(*args, stream)` on `device` (a torch CUDA device) and its current stream."""
-    if device.index is not None and device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return call(fn, *args, torch.cuda.current_stream().cuda_stream)
-    call(fn, *args, torch.cuda.current_stream().cuda_stream)
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return call(fn, *args, _stream_of(index))
+    call(fn, *args, _stream_of(index))

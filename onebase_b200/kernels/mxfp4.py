@@ -32,9 +32,9 @@ def quantize(x: torch.Tensor, codes: Optional[torch.Tensor] = None, scales: Opti
     K = shape[-1]
     given = codes is not None or scales is not None
     if codes is None:
-        codes = torch.empty((*shape[:-1], K // 2), dtype=torch.uint8, device=x.device)
+        codes = x.new_empty((*shape[:-1], K // 2), dtype=torch.uint8)
     if scales is None:
-        scales = torch.empty((*shape[:-1], K // BLOCK), dtype=torch.uint8, device=x.device)
+        scales = x.new_empty((*shape[:-1], K // BLOCK), dtype=torch.uint8)
     if given:
         _check_codes(codes, scales, shape, x.device)
     src = x
@@ -60,7 +60,7 @@ def dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = t
     if out is None:
         if dtype not in _DTYPE:
             raise ValueError("mxfp4.dequantize: dtype must be bf16, fp16 or fp32")
-        out = torch.empty(shape, dtype=dtype, device=codes.device)
+        out = codes.new_empty(shape, dtype=dtype)
     elif out.shape != shape or out.dtype not in _DTYPE or out.device != codes.device or out.stride(-1) != 1 or \
             not (out.dim() == 2 or out.is_contiguous()):
         raise ValueError("mxfp4.dequantize: out must be bf16, fp16 or fp32 of the codes' shape and device, rows dense")

@@ -19,7 +19,8 @@ import torch
 
 from onebase_b200 import _lib
 
-_DTYPE = {torch.bfloat16: _lib.OB_DTYPE_BF16, torch.float16: _lib.OB_DTYPE_F16, torch.float32: _lib.OB_DTYPE_F32}
+_ROWS = {torch.bfloat16: _lib.OB_DTYPE_BF16, torch.float16: _lib.OB_DTYPE_F16}
+_WEIGHT = {**_ROWS, torch.float32: _lib.OB_DTYPE_F32}
 _QUANT = {None: _lib.OB_QUANT_NONE, "fp8": _lib.OB_QUANT_FP8, "mxfp4": _lib.OB_QUANT_MXFP4}
 
 
@@ -30,8 +31,9 @@ class NormOut(NamedTuple):
     scales: Optional[torch.Tensor]     # "fp8": fp32 [...]; "mxfp4": exponent + 127, uint8 [..., K/32]
 
 
-def _strides(t: torch.Tensor) -> tuple[int, int]:
-    return t.stride(0), (t.stride(1) if t.dim() == 3 else 0)
+def _rows(t: Optional[torch.Tensor]):
+    """(pointer, stride between tokens, between heads)."""
+    return (None, 0, 0) if t is None else (t.data_ptr(), t.stride(0), t.stride(1) if t.dim() == 3 else 0)
 
 
 def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 1e-6, *, residual: Optional[torch.Tensor] = None,
@@ -41,17 +43,18 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 1e-6,
     None; residual of x's shape and dtype: s = x + residual is returned (in residual_out if given: it may be the residual
     itself) and s is what is normed.  y = (s * weight) / sqrt(mean(s^2) + eps) goes to `out` (it may be x), or nowhere with
     store=False.  quant = "fp8" or "mxfp4" also returns the codes of y before its rounding to 16 bits, with their scales."""
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         raise RuntimeError("onebase_b200 runs on CUDA devices only (there is no CPU path)")
-    if x.dim() not in (2, 3) or x.dtype not in (torch.bfloat16, torch.float16) or x.shape[-1] < 1 or x.stride(-1) != 1 and x.shape[-1] > 1:
+    shape, dims, dtype, device = x.shape, x.dim(), x.dtype, x.device
+    if dims not in (2, 3) or dtype not in _ROWS or shape[-1] < 1 or (x.stride(-1) != 1 and shape[-1] > 1):
         raise ValueError("rms_norm: x must be [M, K] or [M, H, K], bf16 or fp16, its last dimension dense")
     if quant not in _QUANT:
         raise ValueError("rms_norm: quant must be None, 'fp8' or 'mxfp4'")
-    K = x.shape[-1]
-    H = x.shape[1] if x.dim() == 3 else 1
+    K = shape[-1]
+    H = shape[1] if dims == 3 else 1
     if H < 1:
         raise ValueError("rms_norm: x has no heads")
-    if weight is not None and (weight.shape != (K,) or weight.dtype not in (x.dtype, torch.float32) or weight.device != x.device or
+    if weight is not None and (weight.shape != (K,) or weight.dtype not in (dtype, torch.float32) or weight.device != device or
                                not weight.is_contiguous()):
         raise ValueError("rms_norm: weight must be a dense [K] tensor on x's device, of x's dtype or fp32")
     if residual_out is not None and residual is None:
@@ -59,31 +62,20 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 1e-6,
     if out is not None and not store:
         raise ValueError("rms_norm: out with store=False")
     for name, t in (("residual", residual), ("residual_out", residual_out), ("out", out)):
-        if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.device != x.device or t.stride(-1) != 1 and K > 1):
+        if t is not None and (t.shape != shape or t.dtype != dtype or t.device != device or (t.stride(-1) != 1 and K > 1)):
             raise ValueError(f"rms_norm: {name} must have x's shape, dtype and device, its last dimension dense")
-    y = None if not store else torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+    y = None if not store else x.new_empty(shape) if out is None else out
     if residual is not None and residual_out is None:
-        residual_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        residual_out = x.new_empty(shape)
     codes = scales = None
     if quant == "fp8":
-        codes = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-        scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        codes, scales = x.new_empty(shape, dtype=torch.float8_e4m3fn), x.new_empty(shape[:-1], dtype=torch.float32)
     elif quant == "mxfp4":
         if K % 32:
             raise ValueError("rms_norm: MXFP4 codes need K to be a multiple of 32")
-        codes = torch.empty(*x.shape[:-1], K // 2, dtype=torch.uint8, device=x.device)
-        scales = torch.empty(*x.shape[:-1], K // 32, dtype=torch.uint8, device=x.device)
-    n = _lib.ObRmsNorm()
-    n.M, n.H, n.K, n.dtype, n.quant, n.eps = x.shape[0], H, K, _DTYPE[x.dtype], _QUANT[quant], eps
-    n.x, (n.x_ld, n.x_hd) = x.data_ptr(), _strides(x)
-    if weight is not None:
-        n.weight, n.weight_dtype = weight.data_ptr(), _DTYPE[weight.dtype]
-    if residual is not None:
-        n.residual, (n.residual_ld, n.residual_hd) = residual.data_ptr(), _strides(residual)
-        n.residual_out, (n.residual_out_ld, n.residual_out_hd) = residual_out.data_ptr(), _strides(residual_out)
-    if y is not None:
-        n.y, (n.y_ld, n.y_hd) = y.data_ptr(), _strides(y)
-    if codes is not None:
-        n.codes, n.scales = codes.data_ptr(), scales.data_ptr()
-    _lib.call_on(x.device, "ob_rms_norm", C.byref(n))
+        codes, scales = x.new_empty((*shape[:-1], K // 2), dtype=torch.uint8), x.new_empty((*shape[:-1], K // 32), dtype=torch.uint8)
+    n = _lib.ObRmsNorm(shape[0], H, K, _ROWS[dtype], 0 if weight is None else _WEIGHT[weight.dtype], _QUANT[quant], eps,
+                       *_rows(x), None if weight is None else weight.data_ptr(), *_rows(residual), *_rows(residual_out), *_rows(y),
+                       None if codes is None else codes.data_ptr(), None if scales is None else scales.data_ptr())
+    _lib.call_on(device, "ob_rms_norm", C.byref(n))
     return NormOut(y, residual_out, codes, scales)

@@ -130,6 +130,26 @@ __device__ __forceinline__ bool p2_wait(const K2pParams& p, P2Ctrl* c, uint64_t*
     }
 }
 
+// The value in a register of its own from here on.  The epilogue's registers push what the whole kernel uses into local memory, and a
+// role that read it from there in every slot paid more for that than for its MMAs (the launch leaves next to no first-level cache).
+__device__ __forceinline__ uint32_t own_reg(uint32_t v) {
+    asm volatile("mov.b32 %0, %0;" : "+r"(v));
+    return v;
+}
+__device__ __forceinline__ int own_reg(int v) {
+    asm volatile("mov.b32 %0, %0;" : "+r"(v));
+    return v;
+}
+__device__ __forceinline__ uint64_t own_reg(uint64_t v) {
+    asm volatile("mov.b64 %0, %0;" : "+l"(v));
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ T* own_reg(T* v) {
+    asm volatile("mov.b64 %0, %0;" : "+l"(v));
+    return v;
+}
+
 // Two bf16 sums, each the fp32 sum rounded once (as k2_gemm.cu's residual add).
 __device__ __forceinline__ uint32_t add_bf16x2(uint32_t a, uint32_t b) {
     const __nv_bfloat162 r = __floats2bfloat162_rn(bf16_lo(a) + bf16_lo(b), bf16_hi(a) + bf16_hi(b));
@@ -293,15 +313,6 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
                         for (int h = 0; h < kHalves; ++h)
                             tma_load_2d_pair(slot + h * kP2WBytes, &tm_w, bar0, kb * 128, tl.slice_off + row0 + h * 256);
                         tma_load_2d_pair(slot + kXOff, &tm_x, bar0, kb * 128, tl.t0 + (int)rank * 128);
-                        if (FP4) {
-                            // scales, as 8 (MXFP4: 4) x 256-byte rows of a [rows, 256] byte tensor: this CTA's 128 tokens (the
-                            // MMA's A rows), then both 128-feature tiles of W (every CTA needs the scales of all of B's 256 rows in
-                            // its own tensor memory)
-                            uint8_t* sf = slot + kXOff + kP2XBytes;
-                            tma_load_2d_pair(sf, &tm_xsf, bar0, 0, ((tl.m_idx * p.kblocks + kb) * 2 + (int)rank) * (kSf / 256));
-                            tma_load_2d_pair(sf + kSf, &tm_wsf, bar0, 0, (tl.sf_tile * p.kblocks + kb) * (kSf / 256));
-                            tma_load_2d_pair(sf + 2 * kSf, &tm_wsf, bar0, 0, ((tl.sf_tile + 1) * p.kblocks + kb) * (kSf / 256));
-                        }
                         ++kb;
                     } else {
                         const P2Step e = ctrl->meta[i & 1].steps[li];
@@ -329,16 +340,31 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
         }
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
+            uint8_t* const ring_r = own_reg(ring);
+            P2Ctrl* const ctrl_r = own_reg(ctrl);
+            const uint64_t limit_r = own_reg(limit_ns);
+            const uint32_t tmem_r = own_reg(tmem_base);
+            const int pair_r = own_reg(pair), tiles_r = own_reg(n_tiles), pairs_r = own_reg(n_pairs), rc_r = own_reg(rc), kblocks = own_reg(p.kblocks);
+            {
+            uint8_t* const ring = ring_r;
+            P2Ctrl* const ctrl = ctrl_r;
+            const uint64_t limit_ns = limit_r;
+            const uint32_t tmem_base = tmem_r;
+            const int pair = pair_r, n_tiles = tiles_r, n_pairs = pairs_r, rc = rc_r;
             // =========================================================== MMA issuer of the pair
             // A = tokens (each CTA's 128 are its accumulator's lanes), B = features (128 from each CTA per 256-wide half)
-            const uint32_t idesc4 = umma_idesc_nvfp4(256, 256);
             const uint32_t idesc8 = umma_idesc(0, 0, 256, 256);
             const uint32_t idesc16 = umma_idesc(1, 1, 256, 256);
             const uint32_t row_bytes = (uint32_t)rc * 2;      // an expand tile's row: 32, 64 or 128 bytes, swizzled accordingly
             const uint32_t lt = row_bytes == 128 ? 2u : row_bytes == 64 ? 4u : 6u;
             int it = 0, st = 0;
-            uint32_t ph = 0, sf_par = 0, conv_par = 0;        // phase of the slot; per slot: of its scale barrier, of its `conv` barrier
+            uint32_t ph = 0, conv_par = 0;                    // phase of the slot; per slot: of its `conv` barrier
             const uint32_t ring_addr = smem_u32(ring);
+            // NVFP4, MXFP4: what a slot's MMAs need as running values -- the loop's thread issues four MMAs of 128 cycles each per slot and
+            // its own 70 or so instructions must not take longer
+            uint32_t sf_par = 0;                              // phases of the scale barriers, the slot's own in bit 0
+            uint32_t dxl = (uint32_t)umma_smem_desc(ring_addr + kXOff, 1024, 2), dwl = (uint32_t)umma_smem_desc(ring_addr, 1024, 2);
+            uint32_t sft = tmem_base + 256u, sf_bar = smem_u32(ctrl->sf_ready), empty_bar = smem_u32(ctrl->empty);
             const uint64_t d_w0 = umma_smem_desc(ring_addr, 1024, 2), d_x0 = umma_smem_desc(ring_addr + kXOff, 1024, 2);
             const uint64_t d_b0 = umma_smem_desc(ring_addr, row_bytes * 8, lt), d_h0 = umma_smem_desc(ring_addr + kXOff, row_bytes * 8, lt);
             uint32_t acc = tmem_base;
@@ -349,36 +375,49 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
                 for (int k = 0; k < 4; ++k)
                     umma_f8f6f4_pair(acc + (uint32_t)(h * 256), dx + (uint64_t)(k * 2), dw + (uint64_t)(k * 2), idesc8, k > 0 ? 1u : first);
             };
-            auto advance = [&]() {
-                umma_commit_pair(&ctrl->empty[st], 3);
+            auto advance = [&](bool k_block) {
+                umma_commit_pair_at(empty_bar, 3);
                 ++it;
-                if (++st == kStages) { st = 0; ph ^= 1u; }
+                if (FP4) {
+                    sf_par = (sf_par >> 1) | (((sf_par & 1u) ^ (k_block ? 1u : 0u)) << (kStages - 1));
+                    dxl += kSlot >> 4;
+                    dwl += kSlot >> 4;
+                    sft += kSfCols;
+                    sf_bar += 8;
+                }
+                empty_bar += 8;
+                if (++st == kStages) {
+                    st = 0;
+                    ph ^= 1u;
+                    if (FP4) {
+                        dxl -= kStages * (kSlot >> 4);
+                        dwl -= kStages * (kSlot >> 4);
+                        sft -= kStages * kSfCols;
+                        sf_bar -= kStages * 8;
+                    }
+                    empty_bar -= kStages * 8;
+                }
             };
             auto k_block = [&](uint32_t first) -> bool {      // `first`: 0 for the tile's first (the accumulator starts there)
                 if (FP4) {
                     // the scale copier saw both CTAs' operands land before it copied: one wait covers data and scales; the
                     // barrier completes once per K-BLOCK use of the slot -- expand steps pass it by -- so it has its own parity
-                    if (!p2_wait<false>(p, ctrl, &ctrl->sf_ready[st], (sf_par >> st) & 1u, limit_ns, 4, it)) return false;
-                    sf_par ^= 1u << st;
+                    if (!mbar_try_wait_at(sf_bar, sf_par & 1u) && !p2_wait<false>(p, ctrl, &ctrl->sf_ready[st], sf_par & 1u, limit_ns, 4, it)) return false;
                     tc_fence_after();
-                    const uint64_t off = (uint64_t)(uint32_t)(st * (kSlot >> 4));
-                    const uint64_t dx = d_x0 + off, dw = d_w0 + off;
-                    const uint32_t sft = tmem_base + 256u + (uint32_t)(st * kSfCols);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const uint32_t at = MX ? (uint32_t)k / 2u : (uint32_t)k;          // the atom that holds the MMA's scales
-                        const uint32_t ta = sft + at * 4u, tb = sft + 4u * kAtoms + at * 8u;
-                        if (MX)
-                            umma_mxfp4_pair(acc, dx + (uint64_t)(k * 2), dw + (uint64_t)(k * 2), umma_idesc_mxfp4(256, 256, (uint32_t)(k & 1) * 2u), ta,
-                                            tb, k > 0 ? 1u : first);
-                        else umma_nvfp4_pair(acc, dx + (uint64_t)(k * 2), dw + (uint64_t)(k * 2), idesc4, ta, tb, k > 0 ? 1u : first);
+                        const uint32_t ta = sft + at * 4u, tb = sft + 4u * kAtoms + at * 8u, acc_k = k > 0 ? 1u : first;
+                        if (!MX) umma_nvfp4_pair_lo<umma_idesc_nvfp4(256, 256)>(acc, dxl + k * 2, dwl + k * 2, ta, tb, acc_k);
+                        else if (k & 1) umma_mxfp4_pair_lo<umma_idesc_mxfp4(256, 256, 2)>(acc, dxl + k * 2, dwl + k * 2, ta, tb, acc_k);
+                        else umma_mxfp4_pair_lo<umma_idesc_mxfp4(256, 256, 0)>(acc, dxl + k * 2, dwl + k * 2, ta, tb, acc_k);
                     }
                 } else {
                     if (!p2_wait<true>(p, ctrl, &ctrl->full[st], ph, limit_ns, 4, it)) return false;
 #pragma unroll
                     for (int h = 0; h < kHalves; ++h) half_fp8(st, h, first);
                 }
-                advance();
+                advance(true);
                 return true;
             };
             auto expand_step = [&]() -> bool {
@@ -397,7 +436,7 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
                         if (k * 16 < rc)
                             umma_f16_pair(acc + (uint32_t)(h * 256), dh + (uint64_t)(k * 2), db + (uint64_t)(k * 2), idesc16, 1u);
                 }
-                advance();
+                advance(false);
                 return true;
             };
             bool ok = true;
@@ -412,7 +451,7 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
                 if (kHalves == 2) {
                     // The halves of the accumulator come free one after the other: the first ring's worth of k-blocks goes into the
                     // first half while the epilogues still read the second, then into the second.
-                    const int n = min(kStages, p.kblocks);
+                    const int n = min(kStages, kblocks);
                     int s2 = st;
                     uint32_t ph2 = ph;
                     for (int j = 0; j < n && ok; ++j) {
@@ -427,20 +466,21 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
                     if (!ok) break;
                     for (; kb < n; ++kb) {
                         half_fp8(st, 1, kb > 0 ? 1u : 0u);
-                        advance();
+                        advance(true);
                     }
                 }
-                const int lead = STORED ? min(kStages, p.kblocks) : p.kblocks;
+                const int lead = STORED ? min(kStages, kblocks) : kblocks;
                 for (; kb < lead && ok; ++kb) ok = k_block(kb > 0 ? 1u : 0u);
                 if (!ok || !p2_wait<false>(p, ctrl, &ctrl->meta_full[i & 1], (uint32_t)((i >> 1) & 1), limit_ns, 5, it)) { ok = false; break; }
                 const int n_steps = ctrl->meta[i & 1].n_steps;
                 if (STORED) {
-                    P2Walk walk(lead, p.kblocks, n_steps);
+                    P2Walk walk(lead, kblocks, n_steps);
                     for (int q = 0; q < walk.rem && ok; ++q) ok = walk.next_is_step() ? expand_step() : k_block(1u);
                 } else {
                     for (int li = 0; li < n_steps && ok; ++li) ok = expand_step();
                 }
                 if (ok) umma_commit_pair(&ctrl->acc_full[i % kAccBufs], 3);
+            }
             }
         }
         if (STORED && lane == 0 && rank == 1) {
@@ -470,6 +510,49 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
                         mbar_arrive_remote_release(cluster_peer_addr(smem_u32(&ctrl->conv[st]), 0));
                     }
                     if (++st == kStages) st = 0;
+                }
+            }
+        }
+    } else if (FP4 && warp == 14) {
+        // =========================================================== TMA producer of the block scales (NVFP4, MXFP4): a thread of its own,
+        // because a copy costs its issuer some 130 cycles and five of them per slot bounded the main loop at 780 cycles, whose four MMAs
+        // take 513.  The bytes count on the same barrier, whose phase is rank 0's warp 0's to open.
+        if (lane == 0) {
+            griddep_wait();
+            int st = 0, it = 0;
+            uint32_t ph = 1;
+            bool ok = true;
+            for (int t = pair, i = 0; t < n_tiles && ok; t += n_pairs, ++i) {
+                const P2Tile tl = p2_tile(p, t, m_tiles, kRows);
+                const int lead = STORED ? min(kStages, p.kblocks) : p.kblocks;
+                P2Walk walk(lead, p.kblocks, 0);
+                int total = p.kblocks;
+                for (int q = 0, kb = 0; q < total; ++q, ++it) {
+                    bool step = false;
+                    if (q == lead - 1) {                      // the tile's number of slots, read while it cannot yet be finished without this thread
+                        if (!p2_wait<false>(p, ctrl, &ctrl->meta_full[i & 1], (uint32_t)((i >> 1) & 1), limit_ns, 20, it)) {
+                            ok = false;
+                            break;
+                        }
+                        walk = P2Walk(lead, p.kblocks, ctrl->meta[i & 1].n_steps);
+                        total += walk.n_steps;
+                    }
+                    if (q >= lead) step = walk.next_is_step();
+                    if (!p2_wait<true>(p, ctrl, &ctrl->empty[st], ph, limit_ns, 21, it)) {
+                        ok = false;
+                        break;
+                    }
+                    if (!step) {
+                        // as 8 (MXFP4: 4) x 256-byte rows of a [rows, 256] byte tensor: this CTA's 128 tokens (the MMA's A rows), then both
+                        // 128-feature tiles of W (every CTA needs the scales of all of B's 256 rows in its own tensor memory)
+                        const uint32_t bar0 = cluster_peer_addr(smem_u32(&ctrl->full[st]), 0);
+                        uint8_t* sf = ring + (size_t)st * kSlot + kXOff + kP2XBytes;
+                        tma_load_2d_pair(sf, &tm_xsf, bar0, 0, ((tl.m_idx * p.kblocks + kb) * 2 + (int)rank) * (kSf / 256));
+                        tma_load_2d_pair(sf + kSf, &tm_wsf, bar0, 0, (tl.sf_tile * p.kblocks + kb) * (kSf / 256));
+                        tma_load_2d_pair(sf + 2 * kSf, &tm_wsf, bar0, 0, ((tl.sf_tile + 1) * p.kblocks + kb) * (kSf / 256));
+                        ++kb;
+                    }
+                    if (++st == kStages) { st = 0; ph ^= 1u; }
                 }
             }
         }

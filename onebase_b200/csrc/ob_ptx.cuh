@@ -403,6 +403,59 @@ __device__ __forceinline__ void umma_mxfp4_pair(uint32_t d_tmem, uint64_t a_desc
         "}\n" ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
         : "memory");
 }
+// The same two MMAs for a loop whose issuing thread is what bounds it: descriptors by their low words (the high word is the same for
+// every operand of the kind), everything else known at compile time.
+constexpr uint32_t kUmmaDescHigh128 = (1024u >> 4) | (1u << 14) | (2u << 29);      // of umma_smem_desc(.., 1024, 2)
+template <uint32_t IDESC>
+__device__ __forceinline__ void umma_mxfp4_pair_lo(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t sfa_tmem, uint32_t sfb_tmem,
+                                                   uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        ".reg .b64 a, b;\n"
+        ".reg .b32 i;\n"
+        "mov.b64 a, {%1, %6};\n"
+        "mov.b64 b, {%2, %6};\n"
+        "mov.b32 i, %7;\n"
+        "setp.ne.b32 p, %5, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], a, b, i, [%3], [%4], p;\n"
+        "}\n" ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate), "n"(kUmmaDescHigh128), "n"(IDESC)
+        : "memory");
+}
+template <uint32_t IDESC>
+__device__ __forceinline__ void umma_nvfp4_pair_lo(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t sfa_tmem, uint32_t sfb_tmem,
+                                                   uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        ".reg .b64 a, b;\n"
+        ".reg .b32 i;\n"
+        "mov.b64 a, {%1, %6};\n"
+        "mov.b64 b, {%2, %6};\n"
+        "mov.b32 i, %7;\n"
+        "setp.ne.b32 p, %5, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], a, b, i, [%3], [%4], p;\n"
+        "}\n" ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate), "n"(kUmmaDescHigh128), "n"(IDESC)
+        : "memory");
+}
+// Barrier operations by shared-memory address.
+__device__ __forceinline__ bool mbar_try_wait_at(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ void umma_commit_pair_at(uint32_t bar, uint16_t cta_mask) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(bar), "h"(cta_mask) : "memory");
+}
 // The scale-factor atom copy in both CTAs of the pair: each CTA's shared memory at the descriptor's offset -> its own TMEM.
 __device__ __forceinline__ void tmem_cp_sf_pair(uint32_t taddr, uint64_t smem_desc) {
     asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(smem_desc) : "memory");

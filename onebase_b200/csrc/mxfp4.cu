@@ -2,7 +2,8 @@
 //
 // Four lanes own one block of 32 elements, eight each: a lane loads 16 bytes of a 16-bit tensor (32 of fp32), the block's largest
 // magnitude takes two shuffles, and a lane stores its eight codes as one 32-bit word.  Both directions are bound by memory: 2 bytes
-// read and 17/32 written per bf16 element, or the reverse.
+// read and 17/32 written per bf16 element, or the reverse.  Neither kernel lets its successor start early: what they write may be a
+// projection's weight or adapter, and those are read before the wait on the preceding kernel.
 #include <type_traits>
 
 #include "mxfp4.cuh"
@@ -47,7 +48,6 @@ __device__ __forceinline__ long long mx_offset(long long i, long long total, int
 template <typename T, bool VEC, bool DENSE, int U>
 __global__ void __launch_bounds__(kMxThreads)
 mxfp4_quantize_kernel(const T* __restrict__ x, long long total, int vpr, long long ldx, uint32_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-    griddep_launch_dependents();
     griddep_wait();
     const long long i0 = (long long)blockIdx.x * (kMxThreads * U) + threadIdx.x;
     float v[U][8];
@@ -98,7 +98,6 @@ __device__ __forceinline__ void mx_store8(T* dst, const float (&v)[8]) {
 template <typename T, bool VEC, bool DENSE, int U>
 __global__ void __launch_bounds__(kMxThreads)
 mxfp4_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales, long long total, int vpr, T* __restrict__ out, long long ldo) {
-    griddep_launch_dependents();
     griddep_wait();
     const long long i0 = (long long)blockIdx.x * (kMxThreads * U) + threadIdx.x;
     uint32_t c[U], byte[U];

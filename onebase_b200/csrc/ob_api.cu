@@ -282,6 +282,9 @@ bool small_tiles_win(const ObLayerDesc& d, int m_tiles, long long big_tiles) {
     return d.S == 1 && d.R == 16 && n <= 16 && m_tiles == 1;
 }
 
+// Batches of more tokens than this take the large tiles where layer, call and workspace allow them.
+int big_min_tokens(const ObLayerDesc& d) { return d.base_fmt == OB_BASE_MXFP4 ? kBigTileMinTokensMx : kBigTileMinTokens; }
+
 // `max_split1`: the most shrink splits the caller's workspace holds; the rule for the tensor-core shrink stays within it.  (A split
 // that cfg names does not, and the warp-level shrink's never did: a caller may all-reduce exactly the partials that
 // ob_resolve_tile announces, so a workspace without room for them is refused.)
@@ -338,14 +341,14 @@ int resolve_cfg(const ObLayer* l, int M, const ObTileCfg* cfg, Resolved* r, int 
     int split1 = (cfg && cfg->split1) ? cfg->split1 : 0;
     const int pb = M <= kDecodeTokens ? 1 : 4;
     const int pf = cfg ? cfg->prefill : 0;             // 1 / 2 force the tensor-core / warp-level shrink
-    // Batches of more than 128 tokens take the large-tile GEMM where layer, call and expand list allow it, unless the caller names
+    // Batches of more than 128 tokens (MXFP4 base: 64) take the large-tile GEMM where layer, call and expand list allow it, unless the caller names
     // a token tile (LOWBIT_PREFILL_SMALL_TILES=1 keeps k2_gemm.cu's tiles; LOWBIT_PREFILL_MIN_TILES=n those of launches of
     // fewer than n 256-token tiles; n = 1 by default).
     static const bool no_big = [] { const char* v = std::getenv("LOWBIT_PREFILL_SMALL_TILES"); return v && v[0] == '1'; }();
     static const int min_big_tiles = [] { const char* v = std::getenv("LOWBIT_PREFILL_MIN_TILES"); return v ? std::atoi(v) : 1; }();
     const long long big_tiles = (long long)((M + 255) / 256) * k2_prefill_pair_tiles(d.widths, d.S, 1);
     const long long big_steps = 2LL * (d.L < kMaxTileTenants ? d.L : kMaxTileTenants) * (d.R / l->rc);   // a tile's expand steps at most
-    const bool big_fits = !no_big && l->big_ok && call_takes_big && M > kBigTileMinTokens && !(cfg && cfg->tn) &&
+    const bool big_fits = !no_big && l->big_ok && call_takes_big && M > big_min_tokens(d) && !(cfg && cfg->tn) &&
                           big_steps <= k2_prefill_pair_max_steps() &&
                           (pf == 1 || (big_tiles >= min_big_tiles && !small_tiles_win(d, (M + 255) / 256, big_tiles)));
     // Prefill batches shrink on the tensor cores (LOWBIT_SHRINK_CUDA_CORES=1 keeps the warp-level form): always in front of the
@@ -354,7 +357,7 @@ int resolve_cfg(const ObLayer* l, int M, const ObTileCfg* cfg, Resolved* r, int 
     // for tiles of at most 32 tokens: the GEMM's form for them sums the warp-level shrink's fp32 partials into a table and
     // does not read the tensor-core shrink's finished h.
     static const bool no_mma = [] { const char* v = std::getenv("LOWBIT_SHRINK_CUDA_CORES"); return v && v[0] == '1'; }();
-    const int mma_from = big_fits ? kBigTileMinTokens + 1 : d.lora_fmt == kLoraBf16 ? kMmaShrinkTokens : kMmaShrinkTokensStored;
+    const int mma_from = big_fits ? big_min_tokens(d) + 1 : d.lora_fmt == kLoraBf16 ? kMmaShrinkTokens : kMmaShrinkTokensStored;
     // Nor where its work items would outnumber the workspace's arrival counters (some 130 000 tokens of four slices).
     r->mma_shrink = (!no_mma && pf != 2 && M > kDecodeTokens && (pf == 1 || M >= mma_from) && r->tn > 32 && !b_sharded(d) &&
                      shrink_items(d, M) * d.S <= kCounterSlots) ? 1 : 0;
@@ -752,9 +755,9 @@ int fused_impl(ObLayer* l, const ObBatch* b, void* ws, const ObWorkspaceShape* s
 // What the call's own tensors and workspace say to the large tiles: room for the per-tenant h blocks; rows of y, and of a
 // residual, that take 16-byte accesses; a GPU that holds a pair of them.
 bool call_takes_big(const ObLayer* l, const ObBatch* b, const ObWorkspaceShape* sh) {
-    if (!sh || sh->max_l < l->d.L || b->ldy % 8 != 0 || !aligned16(b->y)) return false;
+    if (!sh || sh->max_l < l->d.L || sh->max_m <= kBigTileMinTokens || b->ldy % 8 != 0 || !aligned16(b->y)) return false;
     if (b->residual != nullptr && (b->ldr % 8 != 0 || !aligned16(b->residual))) return false;
-    return b->M <= kBigTileMinTokens || k2_prefill_pair_capacity() > 0;
+    return b->M <= big_min_tokens(l->d) || k2_prefill_pair_capacity() > 0;
 }
 
 // The size of the large tiles and how many CTA pairs walk them.

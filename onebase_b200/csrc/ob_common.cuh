@@ -18,6 +18,10 @@ constexpr int kMaxTileTenants = 128;  // tenants with a position in one 128-posi
 // gate_up 160 -> 78 us, qkv 119 -> 72, down 162 -> 119, o 102 -> 68 against the warp-level shrink and 128-token tiles.  Up to 128
 // tokens (one small tile) the two are within 10 us of one another, either way.
 constexpr int kBigTileMinTokens = 128;
+// An MXFP4 base already from here: its small tiles hold 64 tokens, so a 65th means a second tile and no K splits (96 tokens, us, small
+// tiles -> large: gate_up, 32 tenants of rank 64 110 -> 80, 4 of rank 16 61 -> 49; down 123 -> 78, 55 -> 51; o 72 -> 51, 31 -> 35, 8 of rank
+// 128 51 -> 57; qkv 94 -> 57, 33 -> 37; at 64 tokens 94 -> 76, 41 -> 49; 72 -> 74, 41 -> 51; 49 -> 49, 25 -> 35; 57 -> 53, 31 -> 37).
+constexpr int kBigTileMinTokensMx = 64;
 constexpr int kMmaShrinkGroup = 4;      // tenants of a 128-position tile per CTA of the tensor-core shrink
 // In front of smaller tiles (layers and calls the large ones do not serve) the tensor-core shrink starts later, from where it
 // measured no slower for any number of tenants and rank (warp-level -> tensor-core, us, 4096 x 4100, FP8 base): bf16 adapters 160

@@ -138,7 +138,7 @@ def test_token_tiles_splits_and_rings(K, M, tn, split2, stages, fmt):
 
 
 @pytest.mark.parametrize("fmt,R", [("bf16", 64), ("bf16", 16), ("fp8", 64), ("nvfp4", 32), ("bf16", 256), ("nvfp4", 128)])
-@pytest.mark.parametrize("K,widths,M,L", [(256, (256,), 129, 4), (1024, (520, 104), 200, 32), (2048, (384, 8, 128), 777, 7), (512, (4096,), 3000, 5), (1056, (264,), 300, 3), (32, (128,), 140, 2), (7392, (136, 256), 260, 4)])
+@pytest.mark.parametrize("K,widths,M,L", [(256, (256,), 129, 4), (1024, (264, 128), 65, 6), (2048, (640,), 128, 3), (1024, (520, 104), 200, 32), (2048, (384, 8, 128), 777, 7), (512, (4096,), 3000, 5), (1056, (264,), 300, 3), (32, (128,), 140, 2), (7392, (136, 256), 260, 4)])
 def test_large_prefill_tiles(K, widths, M, L, fmt, R):
     """The CTA-pair kernel: ragged tokens and slices, several tiles per pair, every storage."""
     d = _case(K, widths, R, L, M, seed=K + M + R)

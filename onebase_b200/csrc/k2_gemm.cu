@@ -329,7 +329,8 @@ k2_kernel(const K2Params p, const __grid_constant__ CUtensorMap tm_w, const __gr
     constexpr int kSf = sf_slot_bytes(BASE), kAtoms = kSf / 512;  // scale factors of 128 rows x one K slot, in 512-byte atoms
     const int sf_bytes = FP4 ? kSf * (1 + p.nblk) : 0;            // W scales + activation scales of one K slot
     const int stage_bytes = kWTileBytes + tn * kBlockK + sf_bytes;
-    const bool small = tn <= 32;                               // decode tiles: h table in shared memory + a builder warp
+    // decode tiles: h table in shared memory + a builder warp (MXFP4 base: 64-token tiles too, where k2_decode_form allows it)
+    const bool small = MX ? p.small != 0 : tn <= 32;
     const int nh = p.nh;                                       // masked H tiles in flight
     const int h_bytes = (int)align_up((size_t)tn * p.rc * 2, 1024);
     uint8_t* ring = smem;
@@ -1184,10 +1185,10 @@ k2_kernel(const K2Params p, const __grid_constant__ CUtensorMap tm_w, const __gr
 
 int k2_fp8_h_tiles(int tn) { return tn <= 16 ? 8 : tn <= 32 ? 4 : 2; }
 
-size_t k2_fp8_smem_bytes(int tn, int stages, int rc, int R, int base_fmt) {
+size_t k2_fp8_smem_bytes(int tn, int stages, int rc, int R, int base_fmt, int small) {
     const size_t sf = (size_t)sf_slot_bytes(base_fmt) * (1 + (tn > 128 ? 2 : 1));
     const size_t aux = (size_t)k2_fp8_h_tiles(tn) * align_up((size_t)tn * rc * 2, 1024) +
-                       (tn <= 32 ? align_up((size_t)tn * R * 2, 1024) : 0);
+                       (small ? align_up((size_t)tn * R * 2, 1024) : 0);
     return 1024 + (size_t)stages * (kWTileBytes + (size_t)tn * kBlockK + sf) + aux + kCtrlBytes;
 }
 

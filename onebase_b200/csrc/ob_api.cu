@@ -11,7 +11,7 @@
 #include "ob_common.cuh"
 
 namespace ob {
-size_t k2_fp8_smem_bytes(int tn, int stages, int rc, int R, int base_fmt);
+size_t k2_fp8_smem_bytes(int tn, int stages, int rc, int R, int base_fmt, int small);
 cudaError_t launch_k2(int base_fmt, const K2Params& p, const CUtensorMap& tm_w, const CUtensorMap& tm_x, const CUtensorMap* tm_b,
                       dim3 grid, size_t smem, int pdl, cudaStream_t stream);
 int k2_fp8_h_tiles(int tn);
@@ -282,6 +282,15 @@ bool small_tiles_win(const ObLayerDesc& d, int m_tiles, long long big_tiles) {
     return d.S == 1 && d.R == 16 && n <= 16 && m_tiles == 1;
 }
 
+// Whether a token tile takes the decode form of the GEMM's expand: K1's partials summed once into a table in shared memory, masked H
+// tiles by a warp of their own -- in place of 128 threads that sum a step's partials again for every step and meet twice in it.  Tiles
+// of up to 32 tokens; for an MXFP4 base of 64 too where a CTA has all of its tile's steps (no K splits) and the table, R up to 64, lets
+// two CTAs share an SM: gate_up, 32 tenants of rank 64, 33 / 48 / 64 tokens 76 / 96 / 90 -> 66 / 72 / 76 us, 16 NVFP4-stored ones 96 / 88 /
+// 96 -> 76 / 76 / 70, 4 of rank 16 41 -> 41.  (Split four ways it is no faster, and slower with stored adapters: down 59-66 -> 68-72.)
+bool k2_decode_form(const ObLayerDesc& d, int tn, int split2, int mma_shrink) {
+    return tn <= kDecodeTokens || (d.base_fmt == OB_BASE_MXFP4 && tn == 64 && split2 == 1 && d.R <= 64 && !mma_shrink);
+}
+
 // Batches of more tokens than this take the large tiles where layer, call and workspace allow them.
 int big_min_tokens(const ObLayerDesc& d) { return d.base_fmt == OB_BASE_MXFP4 ? kBigTileMinTokensMx : kBigTileMinTokens; }
 
@@ -395,6 +404,7 @@ int resolve_cfg(const ObLayer* l, int M, const ObTileCfg* cfg, Resolved* r, int 
         while (r->split1 > 1 && (long long)(r->split1 - 1) * r->k_per_split >= d.K) --r->split1;
     r->pb = pb;
     const int rc = l->rc;
+    const int small = k2_decode_form(d, r->tn, r->split2, r->mma_shrink) ? 1 : 0;
     int stages = r->stream ? r->stages : (cfg && cfg->stages) ? cfg->stages : 0;
     if (r->stream) {
         r->wait_ms = (cfg && cfg->wait_ms > 0) ? (uint32_t)cfg->wait_ms : 2000u;
@@ -404,12 +414,12 @@ int resolve_cfg(const ObLayer* l, int M, const ObTileCfg* cfg, Resolved* r, int 
     if (stages == 0) {   // prefer a footprint that lets two CTAs share an SM (3+ stages; 2+ for 128-token tiles), else the deepest ring that fits
         stages = 12;
         const int floor_stages = r->tn >= 128 ? 2 : 3;
-        while (stages > floor_stages && k2_fp8_smem_bytes(r->tn, stages, rc, d.R, d.base_fmt) > kSmemTwoPerSm) --stages;
-        if (k2_fp8_smem_bytes(r->tn, stages, rc, d.R, d.base_fmt) > kSmemTwoPerSm) stages = 12;
+        while (stages > floor_stages && k2_fp8_smem_bytes(r->tn, stages, rc, d.R, d.base_fmt, small) > kSmemTwoPerSm) --stages;
+        if (k2_fp8_smem_bytes(r->tn, stages, rc, d.R, d.base_fmt, small) > kSmemTwoPerSm) stages = 12;
     }
     if (stages < 2 || stages > 12) return OB_ERR_TILE;
-    while (stages > 2 && k2_fp8_smem_bytes(r->tn, stages, rc, d.R, d.base_fmt) > kSmemLimit) --stages;
-    if (k2_fp8_smem_bytes(r->tn, stages, rc, d.R, d.base_fmt) > kSmemLimit) return OB_ERR_TILE;
+    while (stages > 2 && k2_fp8_smem_bytes(r->tn, stages, rc, d.R, d.base_fmt, small) > kSmemLimit) --stages;
+    if (k2_fp8_smem_bytes(r->tn, stages, rc, d.R, d.base_fmt, small) > kSmemLimit) return OB_ERR_TILE;
     if (fp4)   // TMEM: 2 tn accumulator columns + 32 (MXFP4: 16) scale-factor columns per ring slot, 512 in all
         while (stages > 2 && 2 * r->tn + sf_slot_bytes(d.base_fmt) / 64 * stages > 512) --stages;
     r->stages = stages;
@@ -608,6 +618,7 @@ int k2_prepare(ObLayer* l, const ObBatch* b, void* ws, const ObWorkspaceShape* s
     p.stages = r.stages;
     p.rc = l->rc;
     p.nh = k2_fp8_h_tiles(r.tn);
+    p.small = k2_decode_form(d, r.tn, r.split2, r.mma_shrink) ? 1 : 0;
     p.wsf = static_cast<const uint8_t*>(d.w_sf);
     p.xsf = base + lay.xsf;
     p.alpha = d.alpha;
@@ -648,7 +659,7 @@ int k2_prepare(ObLayer* l, const ObBatch* b, void* ws, const ObWorkspaceShape* s
     if (p.m_fast && l->n_tiles > 65535) return OB_ERR_TOO_LARGE;
     out->grid = p.m_fast ? dim3((unsigned)r.m_tiles, 1u, (unsigned)l->n_tiles)
                          : dim3((unsigned)l->n_tiles, (unsigned)r.split2, (unsigned)r.m_tiles);
-    out->smem = k2_fp8_smem_bytes(r.tn, r.stages, l->rc, d.R, d.base_fmt);
+    out->smem = k2_fp8_smem_bytes(r.tn, r.stages, l->rc, d.R, d.base_fmt, p.small);
     p.cluster_reduce = (scratch == nullptr && fused_ar == nullptr && cluster_reduce_fits(l, r, out->smem)) ? 1 : 0;
     if (fused_ar != nullptr) {      // the all-reduce of a row-parallel layer's output, inside the epilogue
         p.ar_world = fused_ar->world;

@@ -199,6 +199,7 @@ struct K2Params {
     int n_tiles;           // persistent decode kernel: 128-wide output tiles over all slices
     int stages;
     int rc;                // rank chunk per expand step: min(R, 64)
+    int small;             // MXFP4 base: the decode form of the expand (h table and builder warp); the other bases go by tn <= 32
     int nh;                // masked H tiles in flight (expand steps the builder may run ahead of the B tiles)
     int max_m;
     uint32_t wait_ms;

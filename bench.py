@@ -134,6 +134,8 @@ def make_layer(M: int, device, seed: int = 0, base: str = "fp8", lora_fmt: str =
         else:   # NVFP4: timing does not depend on the code values: random nibbles, block scales near 1
             w_q = torch.randint(0, 256, (N, K // 2), device=device, generator=g, dtype=torch.uint8)
             w_sf = torch.randint(0x30, 0x40, (N, K // 16), device=device, generator=g, dtype=torch.uint8).view(torch.float8_e4m3fn)
+            if base == "mxfp4":
+                w_sf = torch.randint(118, 122, (N, K // 32), device=device, generator=g, dtype=torch.uint8)
         del w
         a_st = tuple(((torch.rand(L_SLOTS, 1, RANK, K, device=device, generator=g) * 2 - 1) / K ** 0.5).to(torch.bfloat16)
                      for _ in widths)
@@ -141,6 +143,9 @@ def make_layer(M: int, device, seed: int = 0, base: str = "fp8", lora_fmt: str =
         x = torch.randn(M, K, device=device, generator=g).to(torch.bfloat16)
         if base == "fp8":
             op = VllmFusedFP8LoRA(w_q, s_w, a_st, b_st, max_m=M, lora_fp8=lora_fmt == "fp8", lora_fp4=lora_fmt == "nvfp4")
+        elif base == "mxfp4":
+            from onebase_b200.kernels.mxfp4_lora_vllm import VllmFusedMXFP4LoRA
+            op = VllmFusedMXFP4LoRA(w_q, w_sf, a_st, b_st, max_m=M, lora_fmt=lora_fmt)
         else:
             from onebase_b200.kernels.nvfp4_lora_vllm import VllmFusedNVFP4LoRA
             op = VllmFusedNVFP4LoRA(w_q, w_sf, 2688.0 / 0.1, 2688.0 / 4.0, a_st, b_st, max_m=M, lora_fmt=lora_fmt, rcp_approx=True)
@@ -207,7 +212,8 @@ def profile_case(args, dev) -> None:
 def format_bytes(M: int, distinct: int, base: str, lora_fmt: str) -> int:
     """Algorithmic bytes of one layer pass for a base / adapter storage format: W (+ its block scales), x, y and the distinct
     tenants' A and B with their scales; intermediates excluded."""
-    w_b = 1.0 if base == "fp8" else 0.5625                  # NVFP4: half a byte per code + one scale byte per 16
+    # NVFP4, MXFP4: half a byte per code + one scale byte per 16 or 32
+    w_b = {"fp8": 1.0, "nvfp4": 0.5625, "mxfp4": 0.53125}[base]
     total = 0.0
     for K, widths in PROJECTIONS.values():
         N, S = sum(widths), len(widths)
@@ -264,7 +270,7 @@ def matrix_case(args, dev) -> None:
     """The configurations' grid, one JSON line per cell: base format x adapter storage x batch size."""
     peak, kind = measured_peaks()
     flush = torch.empty(256 * 1024 * 1024, dtype=torch.uint8, device=dev)
-    cells = [("fp8", "bf16"), ("nvfp4", "bf16"), ("fp8", "fp8"), ("nvfp4", "fp8"), ("nvfp4", "nvfp4")]
+    cells = [("fp8", "bf16"), ("nvfp4", "bf16"), ("fp8", "fp8"), ("nvfp4", "fp8"), ("nvfp4", "nvfp4"), ("mxfp4", "bf16"), ("mxfp4", "fp8")]
     sizes = [int(v) for v in args.matrix.split(",")] if args.matrix != "all" else [1, 2, 4, 8, 16, 32, 512, 2048, 8192]
     for base, lora_fmt in cells:
         for M in sizes:
@@ -426,7 +432,7 @@ def main() -> None:
                     help="skip the `reference_gpu` object: the reference's own Triton kernels (out of oracle/_ref) timed on "
                          "the same layer and GPU in a child process, beside the CPU baseline")
     ap.add_argument("--reference-gpu-child", action="store_true", help=argparse.SUPPRESS)
-    ap.add_argument("--base", default="fp8", choices=["fp8", "nvfp4"], help="base format of the --profile case")
+    ap.add_argument("--base", default="fp8", choices=["fp8", "nvfp4", "mxfp4"], help="base format of the --profile case")
     ap.add_argument("--lora-fmt", default="bf16", choices=["bf16", "fp8", "nvfp4"], help="adapter storage of the --profile case")
     ap.add_argument("--tp-form", default="partial", choices=["partial", "sharded"],
                     help="N > 1: row-parallel layers add partial LoRA terms (vLLM's default) or shard the adapters too and "

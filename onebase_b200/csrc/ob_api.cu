@@ -381,6 +381,9 @@ int resolve_cfg(const ObLayer* l, int M, const ObTileCfg* cfg, Resolved* r, int 
         // four splits are one cluster that sums over shared memory; more go through the workspace and their last arriver:
         // unless that divides a long K (1024 elements or more per split), four measured faster
         while (split1 > 4 && d.K / split1 < 1024 && d.R % 16 == 0) split1 /= 2;
+        // (MXFP4 base, whole calls with eight and four: K = 8192, 1000 tokens, 7392 features 88 and 76 us; K = 12288, 4096 features: 200
+        // tokens 73 and 67, 512 72 and 74, 1024 123 and 139, 2048 156 and 189)
+        if (d.base_fmt == OB_BASE_MXFP4 && split1 > 4 && (d.K / split1 < 1536 || M <= 256) && d.R % 16 == 0) split1 = 4;
     }
     if (split1 == 0) {
         const long long units = (long long)((M + pb - 1) / pb) * d.S * (d.R / 8);

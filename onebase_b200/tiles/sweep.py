@@ -1,6 +1,6 @@
 """Sweep the tile choices of the FP8 decode chain on this GPU and write the rows of a tile table.
 
-    python -m onebase_b200.tiles.sweep [--base fp8|nvfp4] [--adapters bf16|fp8|nvfp4] [--out onebase_b200/tiles/qwen3_8b_<base>.jsonl] [--ms 1,2,4,8,16,32]
+    python -m onebase_b200.tiles.sweep [--base fp8|nvfp4|mxfp4] [--adapters bf16|fp8|nvfp4] [--out onebase_b200/tiles/qwen3_8b_<base>.jsonl] [--ms 1,2,4,8,16,32]
 
 For every decode batch size it times one Qwen3-8B decoder layer -- the four projection chains in one CUDA graph, L2
 flushed before each replay, median of the replays -- and walks each projection's choices in turn (GEMM split-K x ring
@@ -73,7 +73,7 @@ def main() -> None:
     ap.add_argument("--out", default=None, help="default: qwen3_8b_<base>.jsonl next to this file")
     ap.add_argument("--ms", default="1,2,4,8,16,32")
     ap.add_argument("--margin", type=float, default=0.02, help="a choice must shorten the layer by this fraction to be kept")
-    ap.add_argument("--base", default="fp8", choices=["fp8", "nvfp4"], help="base format of the swept layer (the rows' fmt key)")
+    ap.add_argument("--base", default="fp8", choices=["fp8", "nvfp4", "mxfp4"], help="base format of the swept layer (the rows' fmt key)")
     ap.add_argument("--adapters", default="bf16", choices=["bf16", "fp8", "nvfp4"],
                     help="storage format of the adapters (the rows' adapters key; bf16 rows carry none)")
     args = ap.parse_args()
@@ -89,6 +89,11 @@ def main() -> None:
             w_q = (torch.randn(N, K, device=dev, generator=g) * 0.5).to(torch.float8_e4m3fn)
             ops[name] = VllmFusedFP8LoRA(w_q, torch.full((1,), 0.01, device=dev), a_st, b_st, max_m=32,
                                          lora_fp8=args.adapters == "fp8", lora_fp4=args.adapters == "nvfp4")
+        elif args.base == "mxfp4":
+            from onebase_b200.kernels.mxfp4_lora_vllm import VllmFusedMXFP4LoRA
+            w_q = torch.randint(0, 256, (N, K // 2), device=dev, generator=g, dtype=torch.uint8)
+            w_sf = torch.randint(118, 122, (N, K // 32), device=dev, generator=g, dtype=torch.uint8)
+            ops[name] = VllmFusedMXFP4LoRA(w_q, w_sf, a_st, b_st, max_m=32, lora_fmt=args.adapters)
         else:   # timing does not depend on the code values: random nibbles, block scales near 1
             from onebase_b200.kernels.nvfp4_lora_vllm import VllmFusedNVFP4LoRA
             w_q = torch.randint(0, 256, (N, K // 2), device=dev, generator=g, dtype=torch.uint8)

@@ -367,3 +367,53 @@ def test_from_weight_and_scale_packing():
             assert int(blk[n:].sum()) == 0 and int(blk[:, K // 32:].sum()) == 0
             tile += 1
         row0 += wd
+
+
+@pytest.mark.parametrize("split2,me", [(1, 0), (3, 1)])
+def test_fused_allreduce_with_a_hand_played_peer(split2, me):
+    """ob_chain_allreduce on this base: the peer's staged partial and announcements are in the buffers before the launch, so nothing
+    waits for another kernel; y is the rank-ordered fp32 sum of both partials, rounded once."""
+    from test_fused_allreduce_gpu import HandComm
+    K, widths, L, M = 1024, (384, 128), 4, 19
+    d = _case(K, widths, 32, L, M, seed=21)
+    op = _op(d, 32)
+    meta, x = device_meta(make_index(d["ids"], L, 32), M), d["x"].cuda()
+    cfg = {"split2": split2}
+    part = op(x, meta, cfg=cfg).clone()
+    torch.cuda.synchronize()
+    hc = HandComm(slot_bytes=32 * 512 * 2, me=me)
+    g = torch.Generator(device="cuda").manual_seed(7)
+    for epoch in (1, 2):
+        theirs = (torch.randn(M, 512, device="cuda", generator=g) * 0.5).to(torch.bfloat16)
+        hc.staged(1 - me, epoch & 1, M, 512).copy_(theirs)
+        hc.tile_flags(me)[1 - me, :4] = epoch
+        y = torch.full_like(part, float("nan"))
+
+        class Peer:
+            comm = hc.comm
+        op(x, meta, out=y, cfg=cfg, allreduce=Peer)
+        _ok(op)
+        parts = [part, theirs] if me == 0 else [theirs, part]
+        assert torch.equal(y, (parts[0].float() + parts[1].float()).to(torch.bfloat16))
+        assert torch.equal(hc.staged(me, epoch & 1, M, 512), part) and bool((hc.tile_flags(1 - me)[me, :4] == epoch).all())
+
+
+def test_two_layers_share_a_workspace_in_two_graphs():
+    """Two captured graphs of two layers over one workspace, replayed in turn on one stream."""
+    d1, d2 = _case(1024, (256,), 16, 3, 20, seed=1), _case(2048, (128, 64), 32, 5, 90, seed=2)
+    op1, op2 = _op(d1, 32), _op(d2, 128)
+    m1, m2 = device_meta(make_index(d1["ids"], 3, 32), 20), device_meta(make_index(d2["ids"], 5, 128), 90)
+    x1, x2 = d1["x"].cuda(), d2["x"].cuda()
+    w1, w2 = op1(x1, m1).clone(), op2(x2, m2).clone()
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for op, x, m in ((op1, x1, m1), (op2, x2, m2)):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(op(x, m))
+        graphs.append(gr)
+    for i in (0, 1, 1, 0, 1, 0):
+        graphs[i].replay()
+    _ok(op1)
+    assert torch.equal(outs[0], w1) and torch.equal(outs[1], w2)
+    check(w2, reference(op2, d2, d2["x"], d2["ids"]))

@@ -79,3 +79,63 @@ def test_oracle_rounds_by_the_table():
     assert byte.tolist() == [[127], [0]]
     assert omx.codes_of(v, byte)[0, :12].tolist() == [7, 0, 1, 2, 2, 4, 4, 6, 6, 7, 10, 15]
     assert omx.scale_bytes(torch.full((1, 32), float("inf"))).item() == 255
+
+
+def test_mxfp4_base_shards():
+    """MXFP4 base under tensor parallelism (shard arithmetic, the oracle standing in for the kernels): column shards concatenate to the
+    unsharded result, row shards -- whose activation codes equal the unsharded ones block for block -- sum to it."""
+    from onebase_b200 import tp
+    from oracle import configs, fp8 as ofp8
+    world = 2
+    d = configs.with_mxfp4_base(configs.draw(256, (128, 64), 16, 4, 11, seed=13, w_std=0.05, b_std=0.05))
+    A, B = ofp8.stack_slices(d["a_stacked"], d["b_stacked"])
+    full = omx.fused_projection(d["x"], d["ids"], d["w_mx"], d["w_mx_sf"], A, B, d["widths"])
+    parts, total = [], torch.zeros_like(full)
+    for rank in range(world):
+        q_r, sf_r, a_r, b_r = tp.shard_column_mxfp4(d["w_mx"], d["w_mx_sf"], d["a_stacked"], d["b_stacked"], world, rank)
+        assert q_r.shape == (96, 128) and sf_r.shape == (96, 8)
+        parts.append(omx.fused_projection(d["x"], d["ids"], q_r, sf_r, *ofp8.stack_slices(a_r, b_r), [t.shape[2] for t in b_r]))
+        q_r, sf_r, a_r, b_r = tp.shard_row_mxfp4(d["w_mx"], d["w_mx_sf"], d["a_stacked"], d["b_stacked"], world, rank)
+        assert q_r.shape == (192, 64) and sf_r.shape == (192, 4) and a_r[0].shape[-1] == 128
+        x_r = tp.shard_input_row(d["x"], world, rank)
+        assert torch.equal(omx.quant(x_r)[1], omx.quant(d["x"])[1][:, rank * 4:(rank + 1) * 4])
+        total += omx.fused_projection(x_r, d["ids"], q_r, sf_r, *ofp8.stack_slices(a_r, b_r), d["widths"])
+    cols, off = [], 0
+    for w in d["widths"]:
+        cols.append(torch.cat([p[:, off // world: (off + w) // world] for p in parts], 1))
+        off += w
+    assert torch.equal(torch.cat(cols, 1), full)
+    # a rank rounds its partial h to bf16: at most half a step of it, against the term's largest value
+    assert float((total - full).abs().max() / full.abs().max()) <= 2 * 2.0 ** -8
+    with pytest.raises(AssertionError):
+        tp.shard_row_mxfp4(d["w_mx"][:, :24], d["w_mx_sf"][:, :1], d["a_stacked"], d["b_stacked"], world, 0)
+
+
+@pytest.mark.parametrize("over,status", [
+    ({"w_sf": None}, -1), ({"alpha": None}, -1), ({"K": 272}, -2), ({"w_q": 0x10004}, -3), ({"w_sf": 0x10004}, -3), ({"base_fmt": 3}, -6),
+])
+def test_mxfp4_layer_refuses(over, status):
+    d = _lib.ObLayerDesc()
+    d.base_fmt, d.lora_fmt = _lib.OB_BASE_MXFP4, 0
+    d.N, d.K, d.S, d.L, d.R, d.max_m = 256, 256, 2, 4, 16, 8
+    d.widths[0], d.widths[1] = 128, 128
+    d.w_q = d.w_sf = d.alpha = FAKE
+    for s in range(2):
+        d.a[s], d.b[s] = FAKE, FAKE
+    for k, v in over.items():
+        setattr(d, k, v)
+    h = C.c_void_p()
+    assert _lib.lib().ob_layer_create(C.byref(d), C.byref(h)) == status and not h.value
+
+
+def test_mxfp4_packed_scale_sizes_and_refusals():
+    lib, n = _lib.lib(), C.c_size_t()
+    w = (C.c_int32 * 2)(200, 72)
+    assert lib.ob_mxfp4_packed_scale_bytes(288, 2, w, C.byref(n)) == 0 and n.value == 3 * 2 * 1024
+    assert lib.ob_mxfp4_packed_scale_bytes(272, 2, w, C.byref(n)) == -2 and lib.ob_mxfp4_packed_scale_bytes(288, 5, w, C.byref(n)) == -2
+    assert lib.ob_mxfp4_packed_scale_bytes(288, 2, w, None) == -1 and lib.ob_mxfp4_packed_scale_bytes(288, 2, None, C.byref(n)) == -1
+    assert lib.ob_mxfp4_pack_scales(FAKE, 288, 2, w, FAKE, 6143, None) == -4
+    assert lib.ob_mxfp4_pack_scales(None, 288, 2, w, FAKE, 6144, None) == -1
+    assert lib.ob_k1_mxfp4(None, None, None, None, None, None) == -1
+    assert lib.ob_k2_mxfp4(None, None, None, None, None, 0, None) == -1
+    assert lib.ob_chain_mxfp4(None, None, None, None, None, None) == -1

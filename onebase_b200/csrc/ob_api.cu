@@ -282,6 +282,27 @@ bool small_tiles_win(const ObLayerDesc& d, int m_tiles, long long big_tiles) {
     return d.S == 1 && d.R == 16 && n <= 16 && m_tiles == 1;
 }
 
+// Clusters of `split2` CTAs of the tile kernel, `smem` bytes of shared memory each, that the current device keeps resident at once.
+int resident_clusters(const ObLayerDesc& d, int split2, size_t smem) {
+    static std::mutex mu;
+    static std::vector<std::pair<unsigned long long, int>> cache;   // (device, formats, split2, smem) -> resident clusters
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    const int base = d.base_fmt, stored = d.lora_fmt == kLoraBf16 ? 0 : 1;
+    const unsigned long long key = ((unsigned long long)dev << 48) | ((unsigned long long)(base * 2 + stored) << 44) |
+                                   ((unsigned long long)split2 << 40) | (unsigned long long)smem;
+    std::lock_guard<std::mutex> g(mu);
+    int n = -1;
+    for (const auto& kv : cache) if (kv.first == key) n = kv.second;
+    if (n < 0) {
+        n = k2_max_active_clusters(base, stored, split2, smem);
+        cache.emplace_back(key, n);
+        if (std::getenv("LOWBIT_VERBOSE"))
+            std::fprintf(stderr, "[onebase_b200] split-K clusters of %d CTAs, %zu B shared memory: %d resident at once\n", split2, smem, n);
+    }
+    return n;
+}
+
 // Whether a token tile takes the decode form of the GEMM's expand: K1's partials summed once into a table in shared memory, masked H
 // tiles by a warp of their own -- in place of 128 threads that sum a step's partials again for every step and meet twice in it.  Tiles
 // of up to 32 tokens; for an MXFP4 base of 64 too where a CTA has all of its tile's steps (no K splits) and the table, R up to 64, lets
@@ -293,6 +314,22 @@ bool k2_decode_form(const ObLayerDesc& d, int tn, int split2, int mma_shrink) {
 
 // Batches of more tokens than this take the large tiles where layer, call and workspace allow them.
 int big_min_tokens(const ObLayerDesc& d) { return d.base_fmt == OB_BASE_MXFP4 ? kBigTileMinTokensMx : kBigTileMinTokens; }
+
+// The ring's depth for a token tile, as asked for (`stages`) or chosen (0); -1: none fits.
+int ring_stages(const ObLayerDesc& d, int tn, int rc, int small, int stages) {
+    if (stages == 0) {   // prefer a footprint that lets two CTAs share an SM (3+ stages; 2+ for 128-token tiles), else the deepest ring that fits
+        stages = 12;
+        const int floor_stages = tn >= 128 ? 2 : 3;
+        while (stages > floor_stages && k2_fp8_smem_bytes(tn, stages, rc, d.R, d.base_fmt, small) > kSmemTwoPerSm) --stages;
+        if (k2_fp8_smem_bytes(tn, stages, rc, d.R, d.base_fmt, small) > kSmemTwoPerSm) stages = 12;
+    }
+    if (stages < 2 || stages > 12) return -1;
+    while (stages > 2 && k2_fp8_smem_bytes(tn, stages, rc, d.R, d.base_fmt, small) > kSmemLimit) --stages;
+    if (k2_fp8_smem_bytes(tn, stages, rc, d.R, d.base_fmt, small) > kSmemLimit) return -1;
+    if (is_fp4(d))   // TMEM: 2 tn accumulator columns + 32 (MXFP4: 16) scale-factor columns per ring slot, 512 in all
+        while (stages > 2 && 2 * tn + sf_slot_bytes(d.base_fmt) / 64 * stages > 512) --stages;
+    return stages;
+}
 
 // `max_split1`: the most shrink splits the caller's workspace holds; the rule for the tensor-core shrink stays within it.  (A split
 // that cfg names does not, and the warp-level shrink's never did: a caller may all-reduce exactly the partials that
@@ -366,11 +403,38 @@ int resolve_cfg(const ObLayer* l, int M, const ObTileCfg* cfg, Resolved* r, int 
     // for tiles of at most 32 tokens: the GEMM's form for them sums the warp-level shrink's fp32 partials into a table and
     // does not read the tensor-core shrink's finished h.
     static const bool no_mma = [] { const char* v = std::getenv("LOWBIT_SHRINK_CUDA_CORES"); return v && v[0] == '1'; }();
-    const int mma_from = big_fits ? big_min_tokens(d) + 1 : d.lora_fmt == kLoraBf16 ? kMmaShrinkTokens : kMmaShrinkTokensStored;
+    // An MXFP4 base's tiles of 33 to 64 tokens take it too for more than 16 bf16 adapters of rank 64 and more on up to 100 feature tiles (32
+    // tenants, 48 tokens, us, warp-level -> tensor-core: qkv 43.1 -> 39.6, down 46.2 -> 40.4, tp8_qkv 46.8 -> 36.2, o 30.4 -> 29.9; but of
+    // rank 16 21.3 -> 31 and 24.7 -> 30.9, 16 tenants of rank 64 33.3 -> 36.4 and 36.5 -> 38.6, and gate_up, 192 tiles, 52.0 -> 60.4).
+    const bool mx_mma = d.base_fmt == OB_BASE_MXFP4 && r->tn == 64 && r->m_tiles == 1 && d.lora_fmt == kLoraBf16 && d.R >= 64 && d.L > 16 && l->n_tiles <= 100;
+    const int mma_from = mx_mma ? kDecodeTokens + 1 : big_fits ? big_min_tokens(d) + 1 : d.lora_fmt == kLoraBf16 ? kMmaShrinkTokens : kMmaShrinkTokensStored;
     // Nor where its work items would outnumber the workspace's arrival counters (some 130 000 tokens of four slices).
     r->mma_shrink = (!no_mma && pf != 2 && M > kDecodeTokens && (pf == 1 || M >= mma_from) && r->tn > 32 && !b_sharded(d) &&
                      shrink_items(d, M) * d.S <= kCounterSlots) ? 1 : 0;
     r->big = big_fits && r->mma_shrink ? 1 : 0;
+    // MXFP4 base, one token tile: half the k-blocks of an FP8 base's row, so the sum over the K splits is a larger part.  As many splits as
+    // form clusters that are all resident (their sum goes over shared memory, and they leave SMs to K1); twice as many for up to 32 tokens
+    // where a CTA would have more than twelve k-blocks; and four in place of two for 33 to 64 tokens where the expand, rank 64 and more, is
+    // split with them (16 FP8-stored ones, 64 tokens: qkv 51.5 -> 43.4, tp4_gate_up 70.0 -> 55.3).
+    // Chains back to back, us, by the rule above and by this: qkv, one token 13.6 -> 12.7, 8 of rank 64 19.5 -> 15.6 with the shrink's
+    // splits (4 -> 2 splits), 48 of rank 16 24.9 -> 21.3; down, one token 18.5 -> 16.3, 8 22.5 -> 16.9, 32 25.9 -> 24.0 (8 -> 4), 48 of rank
+    // 16 34.6 -> 24.7; tp8_gate_up, one token 19.2 -> 17.0 (5 -> 4; 2, which would be clusters, 17.9).
+    if (d.base_fmt == OB_BASE_MXFP4 && r->m_tiles == 1 && r->tn <= 64 && !(cfg && cfg->split2)) {
+        r->split2 = 1;
+        for (const int c : {8, 4, 2}) {
+            const int form = k2_decode_form(d, r->tn, c, r->mma_shrink) ? 1 : 0;
+            const int ring = ring_stages(d, r->tn, l->rc, form, cfg && cfg->stages ? cfg->stages : 0);
+            if (ring > 0 && l->n_tiles * c <= 296 && kblocks / c >= 4 &&
+                l->n_tiles <= resident_clusters(d, c, k2_fp8_smem_bytes(r->tn, ring, l->rc, d.R, d.base_fmt, form))) {
+                r->split2 = c;
+                break;
+            }
+        }
+        const int twice = r->split2 * 2;
+        if (l->n_tiles * twice <= 296 && twice <= 8 &&
+            ((M <= kDecodeTokens && kblocks > 6 * twice) || (M > kDecodeTokens && d.R >= 64 && twice == 4 && kblocks >= 4 * twice)))
+            r->split2 = twice;
+    }
     if (split1 == 0 && r->mma_shrink) {   // one wave of (128-position tile, tenant group, slice, K split) CTAs, at least 256 elements each
         // (tenant groups per tile, where the shrink deals a tile's tenants out to several CTAs: see shrink_group_cap)
         const int cap = shrink_group_cap(d, M);
@@ -384,6 +448,9 @@ int resolve_cfg(const ObLayer* l, int M, const ObTileCfg* cfg, Resolved* r, int 
         // (MXFP4 base, whole calls with eight and four: K = 8192, 1000 tokens, 7392 features 88 and 76 us; K = 12288, 4096 features: 200
         // tokens 73 and 67, 512 72 and 74, 1024 123 and 139, 2048 156 and 189)
         if (d.base_fmt == OB_BASE_MXFP4 && split1 > 4 && (d.K / split1 < 1536 || M <= 256) && d.R % 16 == 0) split1 = 4;
+        // (in front of one tile of up to 64 tokens, which sums them itself, eight: 33 tokens, us, four -> eight: qkv 39.1 -> 37.6,
+        // tp8_qkv 36.8 -> 31.9, tp4_gate_up 49.1 -> 45.8; 64 tokens within 1)
+        if (mx_mma && d.K >= 8 * 512 && tiles * 8 <= 296) split1 = 8;
     }
     if (split1 == 0) {
         const long long units = (long long)((M + pb - 1) / pb) * d.S * (d.R / 8);
@@ -391,11 +458,16 @@ int resolve_cfg(const ObLayer* l, int M, const ObTileCfg* cfg, Resolved* r, int 
         if (pb == 1 && r->stream)   // beside the persistent GEMM the shrink runs as one CTA per SM: one unit per warp of that grid
             while (split1 < 16 && d.K / (split1 * 2) >= 512 && units * split1 * 2 <= (long long)r->grid_s * 8) split1 *= 2;
         else if (pb == 1)   // decode: as many K splits as keep the whole shrink in one wave of the GPU's 2 x 148 CTA slots (8 warps each)
-            while (split1 < 16 && d.K / (split1 * 2) >= 512 && (units * split1 * 2 + 7) / 8 + M <= 296) split1 *= 2;
+            // (an MXFP4 base's GEMM waits less for its weights and more for K1: splits of at least 900 elements leave the SMs' registers to
+            // it sooner.  Chains back to back, us, 512 -> 900: o, 32 tokens, rank 64 17.6 -> 15.9; gate_up, 8 tokens 24.9 -> 23.1, 32 of
+            // rank 16 25.9 -> 23.2; one token the same)
+            while (split1 < 16 && d.K / (split1 * 2) >= (d.base_fmt == OB_BASE_MXFP4 ? 900 : 512) && (units * split1 * 2 + 7) / 8 + M <= 296)
+                split1 *= 2;
         else {         // four positions per warp: two to three waves of warps measured best (each re-reads A through L2);
                        // every CTA of K2 adds the partials again, so a projection with many output tiles wants fewer of them
-            const int cap = l->n_tiles > 100 ? 4 : 16;
-            while (split1 < cap && d.K / (split1 * 2) >= 512 && units * split1 * 2 <= 6144) split1 *= 2;
+            // (MXFP4 base: eight where the tile's sums are made once, see k2_decode_form; 32 tenants, 64 tokens, gate_up 65.6 -> 57 us)
+            const int cap = l->n_tiles <= 100 ? 16 : d.base_fmt == OB_BASE_MXFP4 && k2_decode_form(d, r->tn, r->split2, 0) ? 8 : 4;
+            while (split1 < cap && d.K / (split1 * 2) >= (d.base_fmt == OB_BASE_MXFP4 ? 450 : 512) && units * split1 * 2 <= 6144) split1 *= 2;
         }
     }
     if (r->mma_shrink && !(cfg && cfg->split1))
@@ -414,17 +486,8 @@ int resolve_cfg(const ObLayer* l, int M, const ObTileCfg* cfg, Resolved* r, int 
         r->fused = 0;
         return OB_OK;
     }
-    if (stages == 0) {   // prefer a footprint that lets two CTAs share an SM (3+ stages; 2+ for 128-token tiles), else the deepest ring that fits
-        stages = 12;
-        const int floor_stages = r->tn >= 128 ? 2 : 3;
-        while (stages > floor_stages && k2_fp8_smem_bytes(r->tn, stages, rc, d.R, d.base_fmt, small) > kSmemTwoPerSm) --stages;
-        if (k2_fp8_smem_bytes(r->tn, stages, rc, d.R, d.base_fmt, small) > kSmemTwoPerSm) stages = 12;
-    }
-    if (stages < 2 || stages > 12) return OB_ERR_TILE;
-    while (stages > 2 && k2_fp8_smem_bytes(r->tn, stages, rc, d.R, d.base_fmt, small) > kSmemLimit) --stages;
-    if (k2_fp8_smem_bytes(r->tn, stages, rc, d.R, d.base_fmt, small) > kSmemLimit) return OB_ERR_TILE;
-    if (fp4)   // TMEM: 2 tn accumulator columns + 32 (MXFP4: 16) scale-factor columns per ring slot, 512 in all
-        while (stages > 2 && 2 * r->tn + sf_slot_bytes(d.base_fmt) / 64 * stages > 512) --stages;
+    stages = ring_stages(d, r->tn, rc, small, stages);
+    if (stages < 0) return OB_ERR_TILE;
     r->stages = stages;
     if ((long long)(d.L < r->tn ? d.L : r->tn) * (d.R / rc) > kMaxLoraIters) return OB_ERR_TOO_LARGE;
     r->wait_ms = (cfg && cfg->wait_ms > 0) ? (uint32_t)cfg->wait_ms : 2000u;
@@ -568,23 +631,7 @@ bool cluster_reduce_fits(const ObLayer* l, const Resolved& r, size_t smem) {
     if (force_global || r.split2 < 2 || r.split2 > 8) return false;
     const size_t ring_bytes = (size_t)r.stages * ((size_t)kTileN * kBlockK + (size_t)r.tn * kBlockK);
     if ((size_t)r.tn * kTileN * sizeof(float) > ring_bytes) return false;
-    static std::mutex mu;
-    static std::vector<std::pair<unsigned long long, int>> cache;   // (device, formats, split2, smem) -> resident clusters
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return false;
-    const int base = l->d.base_fmt, stored = l->d.lora_fmt == kLoraBf16 ? 0 : 1;
-    const unsigned long long key = ((unsigned long long)dev << 48) | ((unsigned long long)(base * 2 + stored) << 44) |
-                                   ((unsigned long long)r.split2 << 40) | (unsigned long long)smem;
-    std::lock_guard<std::mutex> g(mu);
-    int n = -1;
-    for (const auto& kv : cache) if (kv.first == key) n = kv.second;
-    if (n < 0) {
-        n = k2_max_active_clusters(base, stored, r.split2, smem);
-        cache.emplace_back(key, n);
-        if (std::getenv("LOWBIT_VERBOSE"))
-            std::fprintf(stderr, "[onebase_b200] split-K clusters of %d CTAs, %zu B shared memory: %d resident at once\n", r.split2, smem, n);
-    }
-    return l->n_tiles <= n;
+    return l->n_tiles <= resident_clusters(l->d, r.split2, smem);
 }
 
 // K2's launch: parameters, tensor map of the quantized activations, grid and shared memory.

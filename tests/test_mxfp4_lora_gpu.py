@@ -137,6 +137,24 @@ def test_token_tiles_splits_and_rings(K, M, tn, split2, stages, fmt):
     assert torch.equal(y, y2)
 
 
+@pytest.mark.parametrize("fmt,R", [("bf16", 64), ("bf16", 16), ("bf16", 256), ("fp8", 128), ("nvfp4", 64)])
+@pytest.mark.parametrize("K,widths,M,L", [(4096, (520, 128, 136), 33, 7), (8192, (1024, 128, 128), 64, 32), (12288, (640,), 47, 3), (512, (2048, 2052), 64, 5), (4096, (8192, 8192), 40, 4), (4064, (24,), 63, 64)])
+def test_one_tile_of_up_to_64_tokens(K, widths, M, L, fmt, R):
+    d = _case(K, widths, R, L, M, seed=M + K)
+    op = _op(d, 64, lora_fmt=fmt)
+    idx = make_index(d["ids"], L, 64)
+    y = op(d["x"].cuda(), device_meta(idx, M))
+    _ok(op)
+    check(y, reference(op, d, d["x"], d["ids"]))
+    for kw in ({"cfg": {"prefill": 1}}, {"cfg": {"prefill": 2}}):
+        y2 = op(d["x"].cuda(), device_meta(idx, M), **kw)
+        _ok(op)
+        check(y2, reference(op, d, d["x"], d["ids"]), kw)
+    y3 = op(d["x"].cuda(), device_meta(idx, M), pdl=False)
+    _ok(op)
+    assert torch.equal(y, y3)
+
+
 @pytest.mark.parametrize("fmt,R", [("bf16", 64), ("bf16", 16), ("fp8", 64), ("nvfp4", 32), ("bf16", 256), ("nvfp4", 128)])
 @pytest.mark.parametrize("K,widths,M,L", [(256, (256,), 129, 4), (1024, (264, 128), 65, 6), (2048, (640,), 128, 3), (1024, (520, 104), 200, 32), (2048, (384, 8, 128), 777, 7), (512, (4096,), 3000, 5), (1056, (264,), 300, 3), (32, (128,), 140, 2), (7392, (136, 256), 260, 4)])
 def test_large_prefill_tiles(K, widths, M, L, fmt, R):

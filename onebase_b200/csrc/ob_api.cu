@@ -305,15 +305,18 @@ int resident_clusters(const ObLayerDesc& d, int split2, size_t smem) {
 
 // Whether a token tile takes the decode form of the GEMM's expand: K1's partials summed once into a table in shared memory, masked H
 // tiles by a warp of their own -- in place of 128 threads that sum a step's partials again for every step and meet twice in it.  Tiles
-// of up to 32 tokens; for an MXFP4 base of 64 too where a CTA has all of its tile's steps (no K splits) and the table, R up to 64, lets
-// two CTAs share an SM: gate_up, 32 tenants of rank 64, 33 / 48 / 64 tokens 76 / 96 / 90 -> 66 / 72 / 76 us, 16 NVFP4-stored ones 96 / 88 /
-// 96 -> 76 / 76 / 70, 4 of rank 16 41 -> 41.  (Split four ways it is no faster, and slower with stored adapters: down 59-66 -> 68-72.)
+// of up to 32 tokens; for an MXFP4 base of 64 too where the table, R up to 64, lets two CTAs share an SM: 64 tokens, us, per step -> table:
+// gate_up, 32 tenants of rank 64 90 -> 76, 16 NVFP4-stored ones 96 -> 70; split two ways qkv, 16 of rank 32 33 -> 28, 16 FP8-stored of rank 64
+// 52 -> 38; four ways o, 32 of rank 16 29 -> 24, down, 16 of rank 64 38.3 -> 34.6, 8 30.7 -> 31.6.  (K1's splits as they were then.)
 bool k2_decode_form(const ObLayerDesc& d, int tn, int split2, int mma_shrink) {
-    return tn <= kDecodeTokens || (d.base_fmt == OB_BASE_MXFP4 && tn == 64 && split2 == 1 && d.R <= 64 && !mma_shrink);
+    return tn <= kDecodeTokens || (d.base_fmt == OB_BASE_MXFP4 && tn == 64 && d.R <= 64 && !mma_shrink);
 }
 
-// Batches of more tokens than this take the large tiles where layer, call and workspace allow them.
-int big_min_tokens(const ObLayerDesc& d) { return d.base_fmt == OB_BASE_MXFP4 ? kBigTileMinTokensMx : kBigTileMinTokens; }
+// Batches of more tokens than this take the large tiles where layer, call and workspace allow them (`forced`: may take them).
+int big_min_tokens(const ObLayerDesc& d, bool forced) {
+    if (d.base_fmt != OB_BASE_MXFP4) return kBigTileMinTokens;
+    return !forced && (d.lora_fmt == kLoraFp8 || (d.S == 1 && d.R <= 64)) ? kBigTileMinTokens : kBigTileMinTokensMx;
+}
 
 // The ring's depth for a token tile, as asked for (`stages`) or chosen (0); -1: none fits.
 int ring_stages(const ObLayerDesc& d, int tn, int rc, int small, int stages) {
@@ -385,7 +388,11 @@ int resolve_cfg(const ObLayer* l, int M, const ObTileCfg* cfg, Resolved* r, int 
     if (split2 > 1 && (long long)l->n_tiles * r->m_tiles > kCounterSlots) return OB_ERR_TOO_LARGE;   // one arrival counter per split tile
     r->split2 = split2;
     int split1 = (cfg && cfg->split1) ? cfg->split1 : 0;
-    const int pb = M <= kDecodeTokens ? 1 : 4;
+    // Positions per warp of the shrink: one for up to 32 tokens, four (which read an adapter's rows once for neighbours of one tenant) for
+    // more; an MXFP4 base's one up to 128: the shrink's latency outweighs the rows' further trips from L2 there (48 tokens, us, four -> one:
+    // qkv, 32 tenants of rank 64 36.0 -> 30.5, 4 of rank 64 24.0 -> 23.7; down 38.3 -> 30.4, 27.9 -> 26.2; tp8_qkv 41.1 -> 34.6, 27.6 ->
+    // 25.1; 96 tokens on two small tiles, 32 of rank 64: gate_up 110 -> 79, down 123 -> 71, o 72 -> 41, qkv 94 -> 53).
+    const int pb = M <= (d.base_fmt == OB_BASE_MXFP4 ? kBigTileMinTokens : kDecodeTokens) ? 1 : 4;
     const int pf = cfg ? cfg->prefill : 0;             // 1 / 2 force the tensor-core / warp-level shrink
     // Batches of more than 128 tokens (MXFP4 base: 64) take the large-tile GEMM where layer, call and expand list allow it, unless the caller names
     // a token tile (LOWBIT_PREFILL_SMALL_TILES=1 keeps k2_gemm.cu's tiles; LOWBIT_PREFILL_MIN_TILES=n those of launches of
@@ -394,7 +401,7 @@ int resolve_cfg(const ObLayer* l, int M, const ObTileCfg* cfg, Resolved* r, int 
     static const int min_big_tiles = [] { const char* v = std::getenv("LOWBIT_PREFILL_MIN_TILES"); return v ? std::atoi(v) : 1; }();
     const long long big_tiles = (long long)((M + 255) / 256) * k2_prefill_pair_tiles(d.widths, d.S, 1);
     const long long big_steps = 2LL * (d.L < kMaxTileTenants ? d.L : kMaxTileTenants) * (d.R / l->rc);   // a tile's expand steps at most
-    const bool big_fits = !no_big && l->big_ok && call_takes_big && M > big_min_tokens(d) && !(cfg && cfg->tn) &&
+    const bool big_fits = !no_big && l->big_ok && call_takes_big && M > big_min_tokens(d, pf == 1) && !(cfg && cfg->tn) &&
                           big_steps <= k2_prefill_pair_max_steps() &&
                           (pf == 1 || (big_tiles >= min_big_tiles && !small_tiles_win(d, (M + 255) / 256, big_tiles)));
     // Prefill batches shrink on the tensor cores (LOWBIT_SHRINK_CUDA_CORES=1 keeps the warp-level form): always in front of the
@@ -403,22 +410,18 @@ int resolve_cfg(const ObLayer* l, int M, const ObTileCfg* cfg, Resolved* r, int 
     // for tiles of at most 32 tokens: the GEMM's form for them sums the warp-level shrink's fp32 partials into a table and
     // does not read the tensor-core shrink's finished h.
     static const bool no_mma = [] { const char* v = std::getenv("LOWBIT_SHRINK_CUDA_CORES"); return v && v[0] == '1'; }();
-    // An MXFP4 base's tiles of 33 to 64 tokens take it too for more than 16 bf16 adapters of rank 64 and more on up to 100 feature tiles (32
-    // tenants, 48 tokens, us, warp-level -> tensor-core: qkv 43.1 -> 39.6, down 46.2 -> 40.4, tp8_qkv 46.8 -> 36.2, o 30.4 -> 29.9; but of
-    // rank 16 21.3 -> 31 and 24.7 -> 30.9, 16 tenants of rank 64 33.3 -> 36.4 and 36.5 -> 38.6, and gate_up, 192 tiles, 52.0 -> 60.4).
-    const bool mx_mma = d.base_fmt == OB_BASE_MXFP4 && r->tn == 64 && r->m_tiles == 1 && d.lora_fmt == kLoraBf16 && d.R >= 64 && d.L > 16 && l->n_tiles <= 100;
-    const int mma_from = mx_mma ? kDecodeTokens + 1 : big_fits ? big_min_tokens(d) + 1 : d.lora_fmt == kLoraBf16 ? kMmaShrinkTokens : kMmaShrinkTokensStored;
+    const int mma_from = big_fits ? big_min_tokens(d, pf == 1) + 1 : d.lora_fmt == kLoraBf16 ? kMmaShrinkTokens : kMmaShrinkTokensStored;
     // Nor where its work items would outnumber the workspace's arrival counters (some 130 000 tokens of four slices).
     r->mma_shrink = (!no_mma && pf != 2 && M > kDecodeTokens && (pf == 1 || M >= mma_from) && r->tn > 32 && !b_sharded(d) &&
                      shrink_items(d, M) * d.S <= kCounterSlots) ? 1 : 0;
     r->big = big_fits && r->mma_shrink ? 1 : 0;
     // MXFP4 base, one token tile: half the k-blocks of an FP8 base's row, so the sum over the K splits is a larger part.  As many splits as
     // form clusters that are all resident (their sum goes over shared memory, and they leave SMs to K1); twice as many for up to 32 tokens
-    // where a CTA would have more than twelve k-blocks; and four in place of two for 33 to 64 tokens where the expand, rank 64 and more, is
-    // split with them (16 FP8-stored ones, 64 tokens: qkv 51.5 -> 43.4, tp4_gate_up 70.0 -> 55.3).
-    // Chains back to back, us, by the rule above and by this: qkv, one token 13.6 -> 12.7, 8 of rank 64 19.5 -> 15.6 with the shrink's
-    // splits (4 -> 2 splits), 48 of rank 16 24.9 -> 21.3; down, one token 18.5 -> 16.3, 8 22.5 -> 16.9, 32 25.9 -> 24.0 (8 -> 4), 48 of rank
-    // 16 34.6 -> 24.7; tp8_gate_up, one token 19.2 -> 17.0 (5 -> 4; 2, which would be clusters, 17.9).
+    // where a CTA would have more than twelve k-blocks, and four in place of two for 33 to 64 tokens whose expand costs the most, stored
+    // adapters and ranks above 64.  Chains back to back, us, by the rule above and by this: qkv, one token 13.6 -> 12.7, 8 of rank 64 19.5 ->
+    // 15.6 with the shrink's splits (4 -> 2 splits); down, one token 18.5 -> 16.3, 8 22.5 -> 16.9, 32 25.9 -> 24.0 (8 -> 4), 48 of rank 16
+    // 34.6 -> 24.7; tp8_gate_up, one token 19.2 -> 17.0 (5 -> 4; 2, which would be clusters, 17.9); 64 tokens, 32 FP8-stored of rank 64,
+    // 2 -> 4: qkv 41.6 -> 39.1, tp4_gate_up 50.5 -> 45.4.
     if (d.base_fmt == OB_BASE_MXFP4 && r->m_tiles == 1 && r->tn <= 64 && !(cfg && cfg->split2)) {
         r->split2 = 1;
         for (const int c : {8, 4, 2}) {
@@ -432,7 +435,7 @@ int resolve_cfg(const ObLayer* l, int M, const ObTileCfg* cfg, Resolved* r, int 
         }
         const int twice = r->split2 * 2;
         if (l->n_tiles * twice <= 296 && twice <= 8 &&
-            ((M <= kDecodeTokens && kblocks > 6 * twice) || (M > kDecodeTokens && d.R >= 64 && twice == 4 && kblocks >= 4 * twice)))
+            ((M <= kDecodeTokens && kblocks > 6 * twice) || (M > kDecodeTokens && (d.R > 64 || d.lora_fmt != kLoraBf16) && twice == 4 && kblocks >= 4 * twice)))
             r->split2 = twice;
     }
     if (split1 == 0 && r->mma_shrink) {   // one wave of (128-position tile, tenant group, slice, K split) CTAs, at least 256 elements each
@@ -448,26 +451,27 @@ int resolve_cfg(const ObLayer* l, int M, const ObTileCfg* cfg, Resolved* r, int 
         // (MXFP4 base, whole calls with eight and four: K = 8192, 1000 tokens, 7392 features 88 and 76 us; K = 12288, 4096 features: 200
         // tokens 73 and 67, 512 72 and 74, 1024 123 and 139, 2048 156 and 189)
         if (d.base_fmt == OB_BASE_MXFP4 && split1 > 4 && (d.K / split1 < 1536 || M <= 256) && d.R % 16 == 0) split1 = 4;
-        // (in front of one tile of up to 64 tokens, which sums them itself, eight: 33 tokens, us, four -> eight: qkv 39.1 -> 37.6,
-        // tp8_qkv 36.8 -> 31.9, tp4_gate_up 49.1 -> 45.8; 64 tokens within 1)
-        if (mx_mma && d.K >= 8 * 512 && tiles * 8 <= 296) split1 = 8;
     }
     if (split1 == 0) {
         const long long units = (long long)((M + pb - 1) / pb) * d.S * (d.R / 8);
         split1 = 1;
         if (pb == 1 && r->stream)   // beside the persistent GEMM the shrink runs as one CTA per SM: one unit per warp of that grid
             while (split1 < 16 && d.K / (split1 * 2) >= 512 && units * split1 * 2 <= (long long)r->grid_s * 8) split1 *= 2;
+        else if (pb == 1 && d.base_fmt == OB_BASE_MXFP4) {
+            // An MXFP4 base's GEMM waits less for its weights and more for K1: splits of at least 900 elements leave the SMs' registers to
+            // it sooner (chains back to back, us, at least 512 -> 900: o, 32 tokens, rank 64 17.6 -> 15.9; gate_up, 8 tokens 24.9 -> 23.1,
+            // 32 of rank 16 25.9 -> 23.2; one token the same).  Up to 32 tokens in one wave as below; for more, two waves (64 tokens, 32
+            // tenants of rank 64, one -> two: down 40.9 -> 34.5, tp4_gate_up 63.0 -> 49.9), unless many feature tiles each sum the
+            // partials for every step (gate_up, 16 of rank 128, 1 -> 2 splits: 79.6 -> 94.7).
+            const long long most = M <= kDecodeTokens || (l->n_tiles > 100 && !k2_decode_form(d, r->tn, r->split2, 0)) ? (296 - M) * 8LL : 4096;
+            while (split1 < 16 && d.K / (split1 * 2) >= 900 && units * split1 * 2 <= most) split1 *= 2;
+        }
         else if (pb == 1)   // decode: as many K splits as keep the whole shrink in one wave of the GPU's 2 x 148 CTA slots (8 warps each)
-            // (an MXFP4 base's GEMM waits less for its weights and more for K1: splits of at least 900 elements leave the SMs' registers to
-            // it sooner.  Chains back to back, us, 512 -> 900: o, 32 tokens, rank 64 17.6 -> 15.9; gate_up, 8 tokens 24.9 -> 23.1, 32 of
-            // rank 16 25.9 -> 23.2; one token the same)
-            while (split1 < 16 && d.K / (split1 * 2) >= (d.base_fmt == OB_BASE_MXFP4 ? 900 : 512) && (units * split1 * 2 + 7) / 8 + M <= 296)
-                split1 *= 2;
+            while (split1 < 16 && d.K / (split1 * 2) >= 512 && (units * split1 * 2 + 7) / 8 + M <= 296) split1 *= 2;
         else {         // four positions per warp: two to three waves of warps measured best (each re-reads A through L2);
                        // every CTA of K2 adds the partials again, so a projection with many output tiles wants fewer of them
-            // (MXFP4 base: eight where the tile's sums are made once, see k2_decode_form; 32 tenants, 64 tokens, gate_up 65.6 -> 57 us)
-            const int cap = l->n_tiles <= 100 ? 16 : d.base_fmt == OB_BASE_MXFP4 && k2_decode_form(d, r->tn, r->split2, 0) ? 8 : 4;
-            while (split1 < cap && d.K / (split1 * 2) >= (d.base_fmt == OB_BASE_MXFP4 ? 450 : 512) && units * split1 * 2 <= 6144) split1 *= 2;
+            const int cap = l->n_tiles > 100 ? 4 : 16;
+            while (split1 < cap && d.K / (split1 * 2) >= 512 && units * split1 * 2 <= 6144) split1 *= 2;
         }
     }
     if (r->mma_shrink && !(cfg && cfg->split1))
@@ -818,7 +822,7 @@ int fused_impl(ObLayer* l, const ObBatch* b, void* ws, const ObWorkspaceShape* s
 bool call_takes_big(const ObLayer* l, const ObBatch* b, const ObWorkspaceShape* sh) {
     if (!sh || sh->max_l < l->d.L || sh->max_m <= kBigTileMinTokens || b->ldy % 8 != 0 || !aligned16(b->y)) return false;
     if (b->residual != nullptr && (b->ldr % 8 != 0 || !aligned16(b->residual))) return false;
-    return b->M <= big_min_tokens(l->d) || k2_prefill_pair_capacity() > 0;
+    return b->M <= big_min_tokens(l->d, true) || k2_prefill_pair_capacity() > 0;
 }
 
 // The size of the large tiles and how many CTA pairs walk them.

@@ -19,8 +19,11 @@ constexpr int kMaxTileTenants = 128;  // tenants with a position in one 128-posi
 // tokens (one small tile) the two are within 10 us of one another, either way.
 constexpr int kBigTileMinTokens = 128;
 // An MXFP4 base already from here: its small tiles hold 64 tokens, so a 65th means a second tile and no K splits (96 tokens, us, small
-// tiles -> large: gate_up, 32 tenants of rank 64 110 -> 80, 4 of rank 16 61 -> 49; down 123 -> 78, 55 -> 51; o 72 -> 51, 31 -> 35, 8 of rank
-// 128 51 -> 57; qkv 94 -> 57, 33 -> 37; at 64 tokens 94 -> 76, 41 -> 49; 72 -> 74, 41 -> 51; 49 -> 49, 25 -> 35; 57 -> 53, 31 -> 37).
+// tiles -> large: gate_up, 32 tenants of rank 64 79 -> 67, 16 of rank 128 99 -> 81, 4 of rank 16 46 -> 42; qkv 53 -> 51, 75 -> 57, 26 -> 28;
+// tp8_qkv 79 -> 60, 99 -> 84, 37 -> 38) -- but not with FP8-stored adapters, whose conversion the large tiles have too few tiles to hide (32
+// of rank 64: gate_up 103 -> 117, qkv 62 -> 75, down 85 -> 112; 8 of rank 16 53 -> 55, 31 -> 35, 47 -> 72), nor for one slice and ranks up
+// to 64, mostly (down, 32 of rank 64 71 -> 71, 8 of rank 64 56 -> 58, 32 of rank 16 54 -> 62; o 41 -> 42, 29 -> 32, 34 -> 38; tp4_down 58 ->
+// 58, 42 -> 46, 44 -> 50; of rank 128 o 61 -> 52).
 constexpr int kBigTileMinTokensMx = 64;
 constexpr int kMmaShrinkGroup = 4;      // tenants of a 128-position tile per CTA of the tensor-core shrink
 // In front of smaller tiles (layers and calls the large ones do not serve) the tensor-core shrink starts later, from where it

@@ -119,11 +119,19 @@ __global__ void __launch_bounds__(kK1Threads, XOP == OB_X_SILU_MUL ? 4 : 6) k1_q
         const int pos = u / chunks, c = u - pos * chunks;
         const __nv_bfloat16* xr = p.x + (int64_t)position_row(p.meta, pos, p.M, n_all, n_ad) * p.ldx;
         uint4 x[4];
+        __nv_bfloat162 lo = __floats2bfloat162_rn(0.0f, 0.0f), hi = lo;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const int i = c * 128 + q * 32 + lane;
-            if (XOP == OB_X_SILU_MUL) x[q] = i < groups ? silu_mul8_quick(p, xr, i * 8) : make_uint4(0u, 0u, 0u, 0u);
+            if (XOP == OB_X_SILU_MUL) x[q] = i < groups ? silu_mul8_quick(p, xr, i * 8, lo, hi) : make_uint4(0u, 0u, 0u, 0u);
             else x[q] = i < groups ? __ldg(reinterpret_cast<const uint4*>(xr) + i) : make_uint4(0u, 0u, 0u, 0u);
+        }
+        if (XOP == OB_X_SILU_MUL && silu_quick_left_range(lo, hi)) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int k = (c * 128 + q * 32 + lane) * 8;
+                if (k < p.K) x[q] = silu_mul8_plain(xr + k, xr + p.K + k);
+            }
         }
         uint32_t* out = reinterpret_cast<uint32_t*>(p.xq + (size_t)pos * (size_t)(p.K >> 1));
         uint4* xo = reinterpret_cast<uint4*>(p.xs + (size_t)pos * (size_t)p.K);

@@ -206,6 +206,31 @@ def test_fused_neighbours(M, silu, residual):
         assert torch.equal(op(x_in.cuda(), meta, silu_mul=silu, residual=yr, out=yr), y)
 
 
+def test_silu_of_infinite_and_far_gates():
+    """The prefill quantizer's cheaper quotient against the decode batch's IEEE division: gates where it would leave its range."""
+    K, M = 1024, 300
+    d = _case(K, (128,), 16, 2, M, seed=5)
+    op = _op(d, 320)
+    idx = make_index(torch.full((M,), -1), 2, 320)
+    x = torch.zeros(M, 2 * K)
+    gates = torch.tensor([float("inf"), float("-inf"), float("nan"), -86.5, -87.5, -88.0, -88.5, -89.0, -120.0, -3e38, 3e38, -0.0, 1e-40, -1e-40])
+    ups = torch.tensor([1.0, -2.0, 3e38, 2.0 ** 120])
+    x[:, K:] = 1.0
+    for r in range(16):                              # a block of 32 per (gate, up): the gate in its first element
+        for b in range(32):
+            k = r * 32 + b
+            x[r, b * 32], x[r, K + b * 32] = gates[k % len(gates)], ups[(k // len(gates)) % len(ups)]
+    x = x.to(torch.bfloat16).cuda()
+    op(x[:16], device_meta(make_index(torch.full((16,), -1), 2, 320), 16), silu_mul=True)
+    _ok(op)
+    few = [t[:16].clone() for t in op.codes(16)]
+    op(x, device_meta(idx, M), silu_mul=True)
+    _ok(op)
+    many = [t[:16] for t in op.codes(M)]
+    assert torch.equal(few[1], many[1]) and torch.equal(few[0], many[0])
+    assert int((few[1] == 255).sum()) >= 16 * 32 // len(gates) * 2     # (at least the gates of -inf and NaN)
+
+
 @pytest.mark.parametrize("M", [3, 70, 300])
 def test_alpha_scales_and_far_apart_blocks(M):
     """Weight scales over many powers of two, blocks of zeros, an alpha that is no power of two."""

@@ -9,7 +9,8 @@
 // with the store's last bit.  max|y| needs no second pass over the row: rounding and the product with a positive number are
 // monotone, so max|y| = max|s w| / sqrt(..) and both reductions run together.
 //
-// A NaN (or an infinity) in a row makes its sum of squares one, and with it every y, the scale and every code of the row.
+// A NaN in a row makes every y, the scale and every code of the row one.  An infinity makes 1 / sqrt(..) zero: the row's y is NaN there and
+// 0 elsewhere, an FP8 row's scale and codes are NaN.
 #include <type_traits>
 
 #include "mxfp4.cuh"
@@ -85,7 +86,6 @@ __device__ __forceinline__ float norm_rstd(float sum, const ObRmsNorm& p) { retu
 // Any row, element by element: G threads, NE elements each held in registers (NE = 0: the row is read twice instead).
 template <typename T, int G, int NE>
 __global__ void __launch_bounds__(norm_block(G)) rms_norm_any_kernel(const ObRmsNorm p) {
-    griddep_launch_dependents();
     constexpr int kRows = norm_block(G) / G;
     const int t = threadIdx.x % G, lane = threadIdx.x & 31;
     const long long row = (long long)blockIdx.x * kRows + threadIdx.x / G;
@@ -96,6 +96,7 @@ __global__ void __launch_bounds__(norm_block(G)) rms_norm_any_kernel(const ObRms
     const T* r = reinterpret_cast<const T*>(a.r);
     const bool w32 = p.weight_dtype == OB_DTYPE_F32;
     griddep_wait();
+    griddep_launch_dependents();                      // (behind the wait: a successor may read, before its own, what a kernel before this one wrote)
     auto weight = [&](int i) { return !p.weight ? 1.0f : w32 ? __ldg(static_cast<const float*>(p.weight) + i) : to_f(static_cast<const T*>(p.weight)[i]); };
     float s[NE > 0 ? NE : 1];
     float sum = 0.0f, top = 0.0f;
@@ -188,7 +189,6 @@ __device__ __forceinline__ uint4 pack16(const float (&v)[8]) {
 
 template <typename T, int Q, int G, int NV>
 __global__ void __launch_bounds__(norm_block(G)) rms_norm_rows_kernel(const ObRmsNorm p) {
-    griddep_launch_dependents();
     constexpr int kRows = norm_block(G) / G;          // rows of a CTA
     const int t = threadIdx.x % G;
     const long long row = (long long)blockIdx.x * kRows + threadIdx.x / G;
@@ -197,6 +197,7 @@ __global__ void __launch_bounds__(norm_block(G)) rms_norm_rows_kernel(const ObRm
     const int nvec = live ? p.K >> 3 : 0;
     const bool w32 = p.weight_dtype == OB_DTYPE_F32;
     griddep_wait();
+    griddep_launch_dependents();                      // (behind the wait, as above)
     uint4 xv[NV], rv[NV];
     float s[NV][8];
 #pragma unroll

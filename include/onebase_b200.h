@@ -123,7 +123,7 @@ typedef struct ObBatch {
     int64_t ldr;
     /*   x_op = OB_X_QUANTIZED   x has been quantized already (ob_rms_norm, ob_mxfp4_quantize): K1 takes these codes into its
      *        order instead of making its own, and x itself -- still [M, K] bf16 -- is what the adapters multiply.  FP8 base:
-     *        x_codes [M, K] e4m3, x_scales [M] fp32; MXFP4 base: x_codes [M, K/2], x_scales [M, K/32]; dense, x_codes 16-byte aligned.
+     *        x_codes [M, K] e4m3, x_scales [M] fp32, above zero; MXFP4 base: x_codes [M, K/2], x_scales [M, K/32]; dense, x_codes 16-byte aligned.
      *        The NVFP4 base refuses it.  Not read under the other values of x_op. */
     const void* x_codes;
     const void* x_scales;

@@ -244,6 +244,9 @@ class VllmFusedFP8LoRA:
         K1 (down_proj).  residual = [M, N] bf16: K2 stores y + residual, the new residual stream (o_proj, down_proj).
         quantized = (codes, scales): x's codes in the base's format (rms_norm's, mxfp4.quantize's), which K1 takes instead of
         quantizing x; x itself is what the adapters multiply."""
+        if x.device.index != torch.cuda.current_device():    # (launches and the occupancy queries behind them go to the current one)
+            with torch.cuda.device(x.device):
+                return self(x, meta_args, out, cfg, pdl, shrink, gemm, allreduce, silu_mul, residual, quantized)
         b, y = self._batch(x, meta_args, out, silu_mul, residual, quantized)
         t = self.tile(b.M, cfg)
         ws, sh = C.c_void_p(self.scratch.ptr), C.byref(self.scratch.shape)

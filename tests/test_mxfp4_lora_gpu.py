@@ -460,3 +460,34 @@ def test_two_layers_share_a_workspace_in_two_graphs():
     _ok(op1)
     assert torch.equal(outs[0], w1) and torch.equal(outs[1], w2)
     check(w2, reference(op2, d2, d2["x"], d2["ids"]))
+
+
+def test_calls_from_another_current_device(monkeypatch):
+    """Each entry makes its tensors' device current for the launch and leaves the caller's as it was."""
+    from onebase_b200.kernels.mxfp4 import dequantize, quantize
+    from onebase_b200.kernels.rms_norm import rms_norm
+    d = _case(256, (128,), 16, 2, 5)
+    op = _op(d, 64)
+    x, meta = d["x"].cuda(), device_meta(make_index(d["ids"], 2, 64), 5)
+    want = op(x, meta), rms_norm(x, None).y, quantize(x)[0], dequantize(*quantize(x))
+    state = {"current": 1, "made": []}
+
+    class Guard:
+        def __init__(self, device):
+            self.index = device if isinstance(device, int) else torch.device(device).index
+
+        def __enter__(self):
+            self.before, state["current"] = state["current"], self.index
+            state["made"].append(self.index)
+
+        def __exit__(self, *exc):
+            state["current"] = self.before
+
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: state["current"])
+    codes, scales = quantize(x)
+    got = op(x, meta), rms_norm(x, None).y, codes, dequantize(codes, scales)
+    monkeypatch.undo()
+    _ok(op)
+    assert state["made"] == [0] * 4 and state["current"] == 1
+    assert all(torch.equal(a, b) for a, b in zip(want, got))

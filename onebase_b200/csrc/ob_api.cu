@@ -461,7 +461,7 @@ int resolve_cfg(const ObLayer* l, int M, const ObTileCfg* cfg, Resolved* r, int 
             // An MXFP4 base's GEMM waits less for its weights and more for K1: splits of at least 900 elements leave the SMs' registers to
             // it sooner (chains back to back, us, at least 512 -> 900: o, 32 tokens, rank 64 17.6 -> 15.9; gate_up, 8 tokens 24.9 -> 23.1,
             // 32 of rank 16 25.9 -> 23.2; one token the same).  Up to 32 tokens about a wave of 300 CTAs' warps (tp8_qkv, 23 tokens of rank
-            // 128, 1 -> 2 splits, 2208 warps: 31.4 -> 25.4; qkv, 32 of rank 64, FP8-stored, 2 -> 4, 3072 warps: 25.8 -> 26.8); for more, two
+            // 128, 1 -> 2 splits, 2208 warps: 31.4 -> 25.4; qkv, 32 of rank 64, FP8-stored, 2 -> 4, some 3000 warps: 25.8 -> 26.8); for more, two
             // waves (64 tokens, 32 tenants of rank 64, one -> two: down 40.9 -> 34.5, tp4_gate_up 63.0 -> 49.9), unless many feature tiles
             // each sum the partials for every step (gate_up, 16 of rank 128, 1 -> 2 splits: 79.6 -> 94.7).
             const long long most = M <= kDecodeTokens || (l->n_tiles > 100 && !k2_decode_form(d, r->tn, r->split2, 0)) ? 2400 : 4096;

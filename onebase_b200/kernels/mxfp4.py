@@ -17,9 +17,9 @@ _DTYPE = {torch.bfloat16: _lib.OB_DTYPE_BF16, torch.float16: _lib.OB_DTYPE_F16, 
 
 def _check_codes(codes: torch.Tensor, scales: torch.Tensor, shape, device) -> None:
     K = shape[-1]
-    for name, t, want in (("codes", codes, (*shape[:-1], K // 2)), ("scales", scales, (*shape[:-1], K // BLOCK))):
+    for t, want in ((codes, (*shape[:-1], K // 2)), (scales, (*shape[:-1], K // BLOCK))):
         if t.dtype != torch.uint8 or t.shape != want or t.device != device or not t.is_contiguous():
-            raise ValueError(f"mxfp4: {name} must be a dense uint8 tensor of shape {tuple(want)} on {device}")
+            raise ValueError(f"mxfp4: codes and scales must be dense uint8 tensors, here one of shape {tuple(want)} on {device}")
 
 
 def quantize(x: torch.Tensor, codes: Optional[torch.Tensor] = None, scales: Optional[torch.Tensor] = None):
@@ -37,12 +37,13 @@ def quantize(x: torch.Tensor, codes: Optional[torch.Tensor] = None, scales: Opti
         scales = x.new_empty((*shape[:-1], K // BLOCK), dtype=torch.uint8)
     if given:
         _check_codes(codes, scales, shape, x.device)
-    src = x
-    if x.dim() != 2 or x.stride(1) != 1:               # rows of the last dimension; a copy where the leading dimensions do not merge
+    src, st = x, x.stride()
+    if len(st) != 2 or st[1] != 1:               # rows of the last dimension; a copy where the leading dimensions do not merge
         src = x.reshape(-1, K)
         if src.stride(1) != 1:
             src = src.contiguous()
-    _lib.call_on(x.device, "ob_mxfp4_quantize", src.data_ptr(), _DTYPE[x.dtype], src.shape[0], K, src.stride(0), codes.data_ptr(),
+        shape, st = src.shape, src.stride()
+    _lib.call_on(x.device, "ob_mxfp4_quantize", src.data_ptr(), _DTYPE[x.dtype], shape[0], K, st[0], codes.data_ptr(),
                  scales.data_ptr())
     return codes, scales
 

@@ -31,9 +31,18 @@ class NormOut(NamedTuple):
     scales: Optional[torch.Tensor]     # "fp8": fp32 [...]; "mxfp4": exponent + 127, uint8 [..., K/32]
 
 
-def _rows(t: Optional[torch.Tensor]):
+_NO_ROWS = (None, 0, 0)
+
+
+def _rows(t: torch.Tensor, dims: int):
     """(pointer, stride between tokens, between heads)."""
-    return (None, 0, 0) if t is None else (t.data_ptr(), t.stride(0), t.stride(1) if t.dim() == 3 else 0)
+    st = t.stride()
+    return t.data_ptr(), st[0], st[1] if dims == 3 else 0
+
+
+def _like(name: str, t: torch.Tensor, shape, dtype, device) -> None:
+    if t.shape != shape or t.dtype != dtype or t.device != device or (t.stride(-1) != 1 and shape[-1] > 1):
+        raise ValueError(f"rms_norm: {name} must have x's shape, dtype and device, its last dimension dense")
 
 
 def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 1e-6, *, residual: Optional[torch.Tensor] = None,
@@ -61,12 +70,15 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 1e-6,
         raise ValueError("rms_norm: residual_out without a residual")
     if out is not None and not store:
         raise ValueError("rms_norm: out with store=False")
-    for name, t in (("residual", residual), ("residual_out", residual_out), ("out", out)):
-        if t is not None and (t.shape != shape or t.dtype != dtype or t.device != device or (t.stride(-1) != 1 and K > 1)):
-            raise ValueError(f"rms_norm: {name} must have x's shape, dtype and device, its last dimension dense")
+    if out is not None:
+        _like("out", out, shape, dtype, device)
+    if residual_out is not None:
+        _like("residual_out", residual_out, shape, dtype, device)
     y = None if not store else x.new_empty(shape) if out is None else out
-    if residual is not None and residual_out is None:
-        residual_out = x.new_empty(shape)
+    if residual is not None:
+        _like("residual", residual, shape, dtype, device)
+        if residual_out is None:
+            residual_out = x.new_empty(shape)
     codes = scales = None
     if quant == "fp8":
         codes, scales = x.new_empty(shape, dtype=torch.float8_e4m3fn), x.new_empty(shape[:-1], dtype=torch.float32)
@@ -75,7 +87,10 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 1e-6,
             raise ValueError("rms_norm: MXFP4 codes need K to be a multiple of 32")
         codes, scales = x.new_empty((*shape[:-1], K // 2), dtype=torch.uint8), x.new_empty((*shape[:-1], K // 32), dtype=torch.uint8)
     n = _lib.ObRmsNorm(shape[0], H, K, _ROWS[dtype], 0 if weight is None else _WEIGHT[weight.dtype], _QUANT[quant], eps,
-                       *_rows(x), None if weight is None else weight.data_ptr(), *_rows(residual), *_rows(residual_out), *_rows(y),
+                       *_rows(x, dims), None if weight is None else weight.data_ptr(),
+                       *(_NO_ROWS if residual is None else _rows(residual, dims)),
+                       *(_NO_ROWS if residual_out is None else _rows(residual_out, dims)),
+                       *(_NO_ROWS if y is None else _rows(y, dims)),
                        None if codes is None else codes.data_ptr(), None if scales is None else scales.data_ptr())
     _lib.call_on(device, "ob_rms_norm", C.byref(n))
     return NormOut(y, residual_out, codes, scales)

@@ -96,7 +96,7 @@ struct P2Ctrl {
     uint64_t acc_empty[2];           // rank 0 only: both CTAs' epilogue warps (16 arrivals)
     uint32_t tmem_base;
     volatile int abort_flag;
-    volatile int b_grant;            // stored adapters: expand steps whose slot the producer has acquired for the epilogue warps to fill
+    volatile int b_grant;            // expand steps whose slot the producer has acquired (stored adapters: for the epilogue warps to fill)
     int go_flag;
     P2Meta meta[2];
 };
@@ -128,6 +128,24 @@ __device__ __forceinline__ bool p2_wait(const K2pParams& p, P2Ctrl* c, uint64_t*
             }
         }
     }
+}
+
+// The scale copiers and the scales' producer put nothing into an expand step's slot, so nothing holds the ring back for them there: one
+// that waited on such a slot's barriers and came two phases late would take the phase in progress for the awaited one and wait for
+// good.  They pass steps by, and before they wait on a k-block's slot again they see by this count, which cannot be mistaken, that the
+// producer has acquired the slots of all `steps` expand steps in front of it: the slot's earlier uses are then over but for the last, and its
+// next one needs their own part, so the slot's free barrier is in the awaited phase or the one behind it.
+__device__ __forceinline__ bool p2_granted(const K2pParams& p, P2Ctrl* c, int steps, uint64_t limit_ns, int where, int it) {
+    if (c->b_grant >= steps) return true;
+    const uint64_t t0 = global_timer_ns();
+    for (uint32_t n = 1; c->b_grant < steps; ++n) {
+        if (c->abort_flag) return false;
+        if ((n & 63u) == 0 && global_timer_ns() - t0 > limit_ns) {
+            p2_timeout(p, c, where, it);
+            return false;
+        }
+    }
+    return true;
 }
 
 // The value in a register of its own from here on.  The epilogue's registers push what the whole kernel uses into local memory, and a
@@ -323,7 +341,7 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
                         const bool in = entry != kP2NoEntry;
                         const int h_row = in ? tl.s * p.max_m + tl.t0 + (int)rank * 128 : p.S * p.max_m + 128;
                         const int h_col = in ? entry * p.R + (int)e.chunk * rc : 0;
-                        if (STORED) {                         // the slot is free: the epilogue warps fill its B tiles
+                        if (STORED || FP4) {                  // the slot is free: the epilogue warps fill its B tiles; p2_granted counts it
                             __threadfence_block();
                             ctrl->b_grant = ++granted;
                         }
@@ -519,7 +537,7 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
         // take 513.  The bytes count on the same barrier, whose phase is rank 0's warp 0's to open.
         if (lane == 0) {
             griddep_wait();
-            int st = 0, it = 0;
+            int st = 0, it = 0, steps = 0, last_step = -kStages - 1;      // expand steps so far, the slot count at the last of them
             uint32_t ph = 1;
             bool ok = true;
             for (int t = pair, i = 0; t < n_tiles && ok; t += n_pairs, ++i) {
@@ -538,11 +556,15 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
                         total += walk.n_steps;
                     }
                     if (q >= lead) step = walk.next_is_step();
-                    if (!p2_wait<true>(p, ctrl, &ctrl->empty[st], ph, limit_ns, 21, it)) {
-                        ok = false;
-                        break;
-                    }
-                    if (!step) {
+                    if (step) {
+                        ++steps;
+                        last_step = it;
+                    } else {
+                        if ((it - last_step <= kStages && !p2_granted(p, ctrl, steps, limit_ns, 22, it)) ||
+                            !p2_wait<true>(p, ctrl, &ctrl->empty[st], ph, limit_ns, 21, it)) {
+                            ok = false;
+                            break;
+                        }
                         // as 8 (MXFP4: 4) x 256-byte rows of a [rows, 256] byte tensor: this CTA's 128 tokens (the MMA's A rows), then both
                         // 128-feature tiles of W (every CTA needs the scales of all of B's 256 rows in its own tensor memory)
                         const uint32_t bar0 = cluster_peer_addr(smem_u32(&ctrl->full[st]), 0);
@@ -564,7 +586,7 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
         // copiers 1 and 2 those of the two 128-feature halves of W: four copies (MXFP4: two) each per slot.
         const int cpi = warp == 3 ? 0 : warp - 11;
         if (FP4 && lane == 0 && rank == 0 && cpi < 3) {
-            int it = 0, st = 0;
+            int it = 0, st = 0, steps = 0, last_step = -kStages - 1;      // (as the scales' producer's)
             uint32_t ph = 0;
             bool ok = true;
             for (int t = pair, i = 0; t < n_tiles && ok; t += n_pairs, ++i) {
@@ -579,13 +601,18 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
                 const int total = p.kblocks + walk.n_steps;
                 for (int q = 0; q < total; ++q, ++it) {
                     const bool step = q >= lead && walk.next_is_step();
-                    if (!p2_wait<true>(p, ctrl, &ctrl->full[st], ph, limit_ns, 13, it)) {
-                        ok = false;
-                        break;
-                    }
-                    // (the expand steps' slots carry no scales, but this thread still follows their barriers phase by phase: a
-                    // parity wait entered a whole phase early would pass at once)
-                    if (!step) {
+                    if (step) {
+                        ++steps;
+                        last_step = it;
+                    } else {
+                        // behind expand steps: once the slot's last use is over, its full barrier is in this use's phase (a parity wait
+                        // entered a whole phase early would pass at once)
+                        if ((it - last_step <= kStages && (!p2_granted(p, ctrl, steps, limit_ns, 23, it) ||
+                                                           !p2_wait<true>(p, ctrl, &ctrl->empty[st], ph ^ 1u, limit_ns, 24, it))) ||
+                            !p2_wait<true>(p, ctrl, &ctrl->full[st], ph, limit_ns, 13, it)) {
+                            ok = false;
+                            break;
+                        }
                         tc_fence_after();
                         const uint32_t sfs = smem_u32(ring + (size_t)st * kSlot) + (uint32_t)(kXOff + kP2XBytes);
                         const uint32_t sft = tmem_base + 256u + (uint32_t)(st * kSfCols);

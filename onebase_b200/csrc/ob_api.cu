@@ -821,7 +821,7 @@ int fused_impl(ObLayer* l, const ObBatch* b, void* ws, const ObWorkspaceShape* s
 // What the call's own tensors and workspace say to the large tiles: room for the per-tenant h blocks; rows of y, and of a
 // residual, that take 16-byte accesses; a GPU that holds a pair of them.
 bool call_takes_big(const ObLayer* l, const ObBatch* b, const ObWorkspaceShape* sh) {
-    if (!sh || sh->max_l < l->d.L || sh->max_m <= kBigTileMinTokens || b->ldy % 8 != 0 || !aligned16(b->y)) return false;
+    if (!sh || sh->max_l < l->d.L || b->ldy % 8 != 0 || !aligned16(b->y)) return false;
     if (b->residual != nullptr && (b->ldr % 8 != 0 || !aligned16(b->residual))) return false;
     return b->M <= big_min_tokens(l->d, true) || k2_prefill_pair_capacity() > 0;
 }

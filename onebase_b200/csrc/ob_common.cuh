@@ -83,7 +83,7 @@ __host__ __device__ inline WorkspaceLayout workspace_layout(const ObWorkspaceSha
     l.xs = off;       off = align_up(off + (s.max_m > kDecodeTokens ? (size_t)s.max_m * (size_t)s.max_k * 2 : 0), 1024);
     l.hb = off;       off = align_up(off + (s.max_m > kDecodeTokens ? (size_t)s.max_sr * (size_t)s.max_m * 2 : 0), 1024);
     const size_t lc = s.max_l < kMaxTileTenants ? (s.max_l > 0 ? s.max_l : 0) : kMaxTileTenants;
-    l.hcat = off;     off = align_up(off + (s.max_m > kBigTileMinTokens ? (size_t)s.max_sr * (size_t)s.max_m * lc * 2 : 0), 1024);
+    l.hcat = off;     off = align_up(off + (s.max_m > kBigTileMinTokensMx ? (size_t)s.max_sr * (size_t)s.max_m * lc * 2 : 0), 1024);
     l.total = off;
     return l;
 }

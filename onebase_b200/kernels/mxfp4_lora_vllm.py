@@ -97,7 +97,7 @@ class VllmFusedMXFP4LoRA(VllmFusedFP8LoRA):
         xq = self.scratch.region("xq", M * (K // 2)).view(M, K // 2)
         if tn is None:   # the token tile the library's own rule gave the last call; 256 under the large-tile prefill GEMM
             rt = self.resolved_tile(M)
-            tn = 256 if rt["prefill"] == 1 and self.scratch.shape.max_m > 128 else rt["tn"]   # (a smaller workspace has no room for it)
+            tn = 256 if rt["prefill"] == 1 else rt["tn"]
         nblk = 2 if tn > 128 else 1
         kslots = (K + 255) // 256
         m_tiles = (M + tn - 1) // tn

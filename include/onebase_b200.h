@@ -249,6 +249,13 @@ int ob_k2_fp8_static(ObLayer* layer, const ObBatch* batch, void* workspace, cons
 int ob_chain_fp8(ObLayer* layer, const ObBatch* batch, void* workspace, const ObWorkspaceShape* shape,
                  const ObTileCfg* cfg, void* cuda_stream);
 
+/* A projection's kernels start beside the launch before them in the stream and read weights, scales and adapters before they wait for
+ * it.  So that launch must not be the one that writes them: behind a kernel or copy that (re)writes an operand in place, and directly in
+ * front of the next projection, call this (one empty launch; capturable).  Any launch without the programmatic attribute in between does as
+ * well.  ob_*_pack_scales and ob_requant_* end with it; ob_mxfp4_quantize and ob_mxfp4_dequantize, whose outputs are activations as often, do
+ * not.  No counterpart in the reference. */
+int ob_operand_fence(void* cuda_stream);
+
 /* The NVFP4-base counterparts of ob_k1_fp8 / ob_k2_fp8 / ob_chain_fp8.  K1 quantizes x to e2m1 codes with one ue4m3
  * scale per 16 elements against the static global scale (vLLM's scaled_fp4_quant recipe) and shrinks; K2 is the
  * block-scaled tcgen05 GEMM (kind::mxf4nvf4, scale factors in TMEM) with the same expand.  Replace the launches of

@@ -116,6 +116,7 @@ SYMBOLS = {
     "ob_nvfp4_packed_scale_bytes": (C.c_int, [C.c_int32, C.c_int32, C.POINTER(C.c_int32), C.POINTER(C.c_size_t)]),
     "ob_nvfp4_pack_scales": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.POINTER(C.c_int32), C.c_void_p, C.c_size_t,
                                        C.c_void_p]),
+    "ob_operand_fence": (C.c_int, [C.c_void_p]),
     "ob_rms_norm": (C.c_int, [C.POINTER(ObRmsNorm), C.c_void_p]),
     "ob_mxfp4_quantize": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p]),
     "ob_mxfp4_dequantize": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p]),

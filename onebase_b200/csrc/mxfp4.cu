@@ -2,8 +2,9 @@
 //
 // Four lanes own one block of 32 elements, eight each: a lane loads 16 bytes of a 16-bit tensor (32 of fp32), the block's largest
 // magnitude takes two shuffles, and a lane stores its eight codes as one 32-bit word.  Both directions are bound by memory: 2 bytes
-// read and 17/32 written per bf16 element, or the reverse.  Neither kernel lets its successor start early: what they write may be a
-// projection's weight or adapter, and those are read before the wait on the preceding kernel.
+// read and 17/32 written per bf16 element, or the reverse.  What they write may be a projection's weight or adapter, which are read
+// before the wait on the preceding kernel: such a write is followed by ob_operand_fence (leaving out the early trigger would not do,
+// as a dependent may also start when the CTAs have left).
 #include <type_traits>
 
 #include "mxfp4.cuh"

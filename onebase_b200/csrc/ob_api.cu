@@ -35,6 +35,7 @@ cudaError_t launch_k2_stream(const K2Params& p, const CUtensorMap& tm_w, const C
                              int grid, size_t smem, int fp4, int pdl, cudaStream_t stream);
 cudaError_t launch_pack_scales(int base_fmt, const uint8_t* linear, int K, int S, const int32_t* widths, uint8_t* packed, size_t bytes,
                                cudaStream_t stream);
+cudaError_t launch_operand_fence(cudaStream_t stream);
 cudaError_t launch_rms_norm(const ObRmsNorm& p, cudaStream_t stream);
 cudaError_t launch_mxfp4_quantize(const void* x, int dtype, long long rows, int K, long long ldx, void* codes, void* scales, cudaStream_t stream);
 cudaError_t launch_mxfp4_dequantize(const void* codes, const void* scales, int dtype, long long rows, int K, void* out, long long ldo,
@@ -1170,6 +1171,12 @@ int ob_mxfp4_pack_scales(const void* w_sf_linear, int32_t K, int32_t S, const in
     if (packed_bytes < need) return OB_ERR_WORKSPACE;
     cudaError_t e = launch_pack_scales(OB_BASE_MXFP4, static_cast<const uint8_t*>(w_sf_linear), K, S, widths, static_cast<uint8_t*>(packed),
                                        need, static_cast<cudaStream_t>(cuda_stream));
+    if (e == cudaSuccess) e = launch_operand_fence(static_cast<cudaStream_t>(cuda_stream));
+    return e == cudaSuccess ? OB_OK : (int)e;
+}
+
+int ob_operand_fence(void* cuda_stream) {
+    cudaError_t e = launch_operand_fence(static_cast<cudaStream_t>(cuda_stream));
     return e == cudaSuccess ? OB_OK : (int)e;
 }
 
@@ -1194,6 +1201,7 @@ int ob_nvfp4_pack_scales(const void* w_sf_linear, int32_t K, int32_t S, const in
     if (packed_bytes < need) return OB_ERR_WORKSPACE;
     cudaError_t e = launch_pack_scales(OB_BASE_NVFP4, static_cast<const uint8_t*>(w_sf_linear), K, S, widths, static_cast<uint8_t*>(packed),
                                        need, static_cast<cudaStream_t>(cuda_stream));
+    if (e == cudaSuccess) e = launch_operand_fence(static_cast<cudaStream_t>(cuda_stream));
     return e == cudaSuccess ? OB_OK : (int)e;
 }
 
@@ -1202,6 +1210,7 @@ int ob_requant_fp8_rows(const void* src, int64_t rows, int32_t cols, void* codes
     if (rows < 1 || rows > 0x7fffffffLL || cols < 8 || cols % 8 != 0) return OB_ERR_SHAPE;
     if (!aligned16(src) || (reinterpret_cast<uintptr_t>(codes) & 7u)) return OB_ERR_ALIGN;
     cudaError_t e = launch_requant_fp8(src, rows, cols, codes, scales, static_cast<cudaStream_t>(cuda_stream));
+    if (e == cudaSuccess) e = launch_operand_fence(static_cast<cudaStream_t>(cuda_stream));
     return e == cudaSuccess ? OB_OK : (int)e;
 }
 
@@ -1213,6 +1222,7 @@ int ob_requant_nvfp4(const void* src, int32_t l, int32_t rows, int32_t cols, voi
         return OB_ERR_ALIGN;
     cudaError_t e = launch_requant_nvfp4(src, l, rows, cols, packed, sf, inv_global, static_cast<unsigned int*>(amax_scratch),
                                          static_cast<cudaStream_t>(cuda_stream));
+    if (e == cudaSuccess) e = launch_operand_fence(static_cast<cudaStream_t>(cuda_stream));
     return e == cudaSuccess ? OB_OK : (int)e;
 }
 

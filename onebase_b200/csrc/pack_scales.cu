@@ -28,6 +28,17 @@ __global__ void pack_scales_kernel(const uint8_t* __restrict__ linear, uint8_t* 
     }
 }
 
+// A launch without work, and without the programmatic attribute: it starts when everything before it in the stream is complete and visible,
+// and a projection behind it -- whose kernels read weights, scales and adapters before their wait on the preceding launch -- starts behind
+// it.  (Directly behind the kernel that wrote an operand, a programmatic dependent may start when that kernel's CTAs have left, and only its
+// wait makes what they wrote visible.)
+__global__ void operand_fence_kernel() {}
+
+cudaError_t launch_operand_fence(cudaStream_t stream) {
+    operand_fence_kernel<<<1, 1, 0, stream>>>();
+    return cudaGetLastError();
+}
+
 cudaError_t launch_pack_scales(int base_fmt, const uint8_t* linear, int K, int S, const int32_t* widths, uint8_t* packed, size_t bytes,
                                cudaStream_t stream) {
     PackArgs a = {};

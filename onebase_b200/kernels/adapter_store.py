@@ -148,8 +148,10 @@ class AdapterStore:
 
     @torch.no_grad()
     def requantize(self, index: int | None = None) -> None:
-        """Refresh slot `index` (all slots if None) of every copy from vLLM's buffers, after vLLM wrote or cleared it."""
+        """Refresh slot `index` (all slots if None) of every copy from vLLM's buffers, after vLLM wrote or cleared it.  The next
+        projection reads what was written (bf16: vLLM's own write of the slot), though it starts beside the launch before it."""
         if self.fmt == "bf16":
+            self._fence()
             return
         if self.staged and index is None:
             raise RuntimeError("with released slots only one slot at a time can be refreshed (from the staging slot)")
@@ -158,3 +160,8 @@ class AdapterStore:
         for s in range(self.S):
             self._a[s].refresh(self.fmt, self.a_stacked[s][src], dst)
             self._b[s].refresh(self.fmt, self.b_stacked[s][src], dst)
+        self._fence()
+
+    def _fence(self) -> None:
+        if self.a_stacked[0].is_cuda:
+            _lib.call_on(self.a_stacked[0].device, "ob_operand_fence")

@@ -270,7 +270,7 @@ class VllmFusedFP8LoRA:
 
     def requantize(self, index: int | None = None) -> None:
         """Refresh the low-precision copy of one slot (or all) from vLLM's bf16 slots after vLLM wrote or cleared it
-        (reference: fp8_lora_vllm.py:504-524).  bf16 adapters are read in place: nothing to do."""
+        (reference: fp8_lora_vllm.py:504-524).  bf16 adapters are read in place: only the order of the write and the next call is seen to."""
         self.store.requantize(index)
 
     def release(self, a_stage, b_stage) -> None:

@@ -23,7 +23,8 @@ def _check_codes(codes: torch.Tensor, scales: torch.Tensor, shape, device) -> No
 
 
 def quantize(x: torch.Tensor, codes: Optional[torch.Tensor] = None, scales: Optional[torch.Tensor] = None):
-    """x [..., K] (bf16, fp16 or fp32, K a multiple of 32) -> (codes, scales), written into the given tensors if any."""
+    """x [..., K] (bf16, fp16 or fp32, K a multiple of 32) -> (codes, scales), written into the given tensors if any (which may be a
+    projection's weight: the next call sees it)."""
     if not x.is_cuda:
         raise RuntimeError("onebase_b200 runs on CUDA devices only (there is no CPU path)")
     shape = x.shape
@@ -45,12 +46,15 @@ def quantize(x: torch.Tensor, codes: Optional[torch.Tensor] = None, scales: Opti
         shape, st = src.shape, src.stride()
     _lib.call_on(x.device, "ob_mxfp4_quantize", src.data_ptr(), _DTYPE[x.dtype], shape[0], K, st[0], codes.data_ptr(),
                  scales.data_ptr())
+    if given:
+        _lib.call_on(x.device, "ob_operand_fence")
     return codes, scales
 
 
 def dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """The values of codes [..., K/2] and scales [..., K/32] as `dtype` (exact in bf16 and fp32 while they are in its range)."""
+    """The values of codes [..., K/2] and scales [..., K/32] as `dtype` (exact in bf16 and fp32 while they are in its range), written
+    into `out` if given (which may be a projection's adapter: the next call sees it)."""
     if not codes.is_cuda:
         raise RuntimeError("onebase_b200 runs on CUDA devices only (there is no CPU path)")
     if codes.dim() < 1 or codes.shape[-1] < BLOCK // 2 or codes.shape[-1] % (BLOCK // 2):
@@ -58,7 +62,8 @@ def dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = t
     K = 2 * codes.shape[-1]
     shape = (*codes.shape[:-1], K)
     _check_codes(codes, scales, shape, codes.device)
-    if out is None:
+    given = out is not None
+    if not given:
         if dtype not in _DTYPE:
             raise ValueError("mxfp4.dequantize: dtype must be bf16, fp16 or fp32")
         out = codes.new_empty(shape, dtype=dtype)
@@ -68,4 +73,6 @@ def dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = t
     dst = out if out.dim() == 2 else out.view(-1, K)
     _lib.call_on(codes.device, "ob_mxfp4_dequantize", codes.data_ptr(), scales.data_ptr(), _DTYPE[out.dtype], dst.shape[0], K,
                  dst.data_ptr(), dst.stride(0))
+    if given:
+        _lib.call_on(codes.device, "ob_operand_fence")
     return out

@@ -2,7 +2,7 @@
 //
 //   s = x + residual                      (fp32; residual_out = s rounded once)
 //   y = (s w) / sqrt(mean(s^2) + eps)     (fp32; y's store rounds once)
-//   FP8:   scale = max(max|y| / 448, 1 / (448 * 512)) per row, codes = e4m3(y / scale), the quotient as a product with the row's 1 / scale
+//   FP8:   scale = max(max|y| / 448, 1 / (448 * 512)) per row, codes = e4m3(y / scale)
 //   MXFP4: per 32 elements, see mxfp4.cuh
 //
 // The codes are rounded from the fp32 y and not from its 16-bit store: one rounding instead of two, and a scale that does not jump
@@ -53,6 +53,14 @@ __device__ __forceinline__ NormRow norm_row(const ObRmsNorm& p, long long row) {
 __device__ __forceinline__ float norm_fp8_scale(float amax) {
     const float sc = __fdiv_rn(amax, kNormFp8Max);
     return sc < kNormMinScale ? kNormMinScale : sc;
+}
+
+// y / scale from the rounded inv = 1 / scale: the product, corrected by its own remainder (Markstein), which is the quotient rounded once
+// -- as the projection's own quantizer divides -- in two more instructions instead of a division's dozen.  The product alone is off by a last
+// bit for a fifth of all y, and where y / scale is a tie of e4m3 that gave another code.
+__device__ __forceinline__ float norm_quotient(float y, float sc, float inv) {
+    const float q = y * inv;
+    return fmaf(-fmaf(q, sc, -y), inv, q);            // (in this form a zero keeps its sign)
 }
 
 // Sum and (FP8) largest magnitude over the G threads of a row.
@@ -129,7 +137,7 @@ __global__ void __launch_bounds__(norm_block(G)) rms_norm_any_kernel(const ObRms
     auto store = [&](int i, float y) {                // every lane of the warp (MXFP4: K % 32 == 0, a warp's lanes are one block's elements)
         if (a.y && i < K) reinterpret_cast<T*>(a.y)[i] = from_f<T>(y);
         if (p.quant == OB_QUANT_FP8) {
-            if (i < K) static_cast<uint8_t*>(p.codes)[row * p.K + i] = (uint8_t)(cvt_e4m3x2(y * inv, 0.0f) & 0xFFu);
+            if (i < K) static_cast<uint8_t*>(p.codes)[row * p.K + i] = (uint8_t)(cvt_e4m3x2(norm_quotient(y, sc, inv), 0.0f) & 0xFFu);
         } else if (p.quant == OB_QUANT_MXFP4) {
             uint32_t m = abs_bits(y);
 #pragma unroll
@@ -249,7 +257,7 @@ __global__ void __launch_bounds__(norm_block(G)) rms_norm_rows_kernel(const ObRm
             if (i < nvec) {
                 uint32_t c[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) c[e] = cvt_e4m3x2(s[q][2 * e] * inv, s[q][2 * e + 1] * inv);
+                for (int e = 0; e < 4; ++e) c[e] = cvt_e4m3x2(norm_quotient(s[q][2 * e], sc, inv), norm_quotient(s[q][2 * e + 1], sc, inv));
                 reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.codes) + row * p.K)[i] = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
             }
         } else if (Q == OB_QUANT_MXFP4) {             // (K % 32 == 0: the four lanes of a block are all in the row, or none is)

@@ -310,8 +310,8 @@ int ob_requant_nvfp4(const void* src, int32_t l, int32_t rows, int32_t cols, voi
  *     OB_QUANT_MXFP4   codes [M * H, K/2] and scales [M * H, K/32] as ob_mxfp4_quantize gives them
  * which ob_chain_fp8 / ob_chain_mxfp4 take as ObBatch.x_codes / x_scales.  Strides are in elements: `*_ld` between tokens, `*_hd`
  * between a token's heads (H = 1: unused).  An output may be the same memory as an input of the same strides, else they must not
- * overlap.  A row that holds a NaN or an infinity has NaN for its scale and codes (and for its y, but for zeros where an infinity divides a
- * number).  One launch, capturable, no workspace; M = 0 does nothing.  No counterpart in the reference, which leaves the norm to
+ * overlap.  A row that holds a NaN has NaN for its y, scales and codes.  One that holds an infinity has NaN there for its y and zeros
+ * elsewhere, NaN for its FP8 scale and codes, and MXFP4 blocks of those y.  One launch, capturable, no workspace; M = 0 does nothing.  No counterpart in the reference, which leaves the norm to
  * vLLM (RMSNorm, vllm/model_executor/layers/layernorm.py). */
 enum { OB_QUANT_NONE = 0, OB_QUANT_FP8 = 1, OB_QUANT_MXFP4 = 2 };
 typedef struct ObRmsNorm {

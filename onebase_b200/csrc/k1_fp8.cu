@@ -102,8 +102,8 @@ __global__ void __launch_bounds__(NT, MIN_CTAS) k1_quant_regs_kernel(const K1Par
 // The MXFP4 base's form of it: a block of 32 elements is all its quantization needs, so a warp takes 1024 elements of a row at a time --
 // four loads per lane (and, with the input transform, four more) in flight -- and walks the batch with the grid's stride; the segment
 // index is read once per warp.  Bound by memory (x read, codes and sorted copy written: 4.5 bytes per element), with the transform by its
-// instructions.  Whole launch, against a CTA per row: 8192 rows of 4096 37 -> 29-33 us; SiLU * mul, 2048 rows of
-// 12288 45 -> 41.
+// instructions; the plain form spills 16 bytes under its bound of six CTAs.  Whole launch, against a CTA per row: 8192 rows of 4096
+// 37 -> 29-33 us; SiLU * mul, 2048 rows of 12288 45 -> 41.
 template <int XOP>
 __global__ void __launch_bounds__(kK1Threads, XOP == OB_X_SILU_MUL ? 4 : 6) k1_quant_mx_kernel(const K1Params p) {
     griddep_launch_dependents();

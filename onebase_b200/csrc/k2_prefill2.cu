@@ -363,142 +363,142 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
             const uint64_t limit_r = own_reg(limit_ns);
             const uint32_t tmem_r = own_reg(tmem_base);
             const int pair_r = own_reg(pair), tiles_r = own_reg(n_tiles), pairs_r = own_reg(n_pairs), rc_r = own_reg(rc), kblocks = own_reg(p.kblocks);
-            {
-            uint8_t* const ring = ring_r;
-            P2Ctrl* const ctrl = ctrl_r;
-            const uint64_t limit_ns = limit_r;
-            const uint32_t tmem_base = tmem_r;
-            const int pair = pair_r, n_tiles = tiles_r, n_pairs = pairs_r, rc = rc_r;
-            // =========================================================== MMA issuer of the pair
-            // A = tokens (each CTA's 128 are its accumulator's lanes), B = features (128 from each CTA per 256-wide half)
-            const uint32_t idesc8 = umma_idesc(0, 0, 256, 256);
-            const uint32_t idesc16 = umma_idesc(1, 1, 256, 256);
-            const uint32_t row_bytes = (uint32_t)rc * 2;      // an expand tile's row: 32, 64 or 128 bytes, swizzled accordingly
-            const uint32_t lt = row_bytes == 128 ? 2u : row_bytes == 64 ? 4u : 6u;
-            int it = 0, st = 0;
-            uint32_t ph = 0, conv_par = 0;                    // phase of the slot; per slot: of its `conv` barrier
-            const uint32_t ring_addr = smem_u32(ring);
-            // NVFP4, MXFP4: what a slot's MMAs need as running values -- the loop's thread issues four MMAs of 128 cycles each per slot and
-            // its own 70 or so instructions must not take longer
-            uint32_t sf_par = 0;                              // phases of the scale barriers, the slot's own in bit 0
-            uint32_t dxl = (uint32_t)umma_smem_desc(ring_addr + kXOff, 1024, 2), dwl = (uint32_t)umma_smem_desc(ring_addr, 1024, 2);
-            uint32_t sft = tmem_base + 256u, sf_bar = smem_u32(ctrl->sf_ready), empty_bar = smem_u32(ctrl->empty);
-            const uint64_t d_w0 = umma_smem_desc(ring_addr, 1024, 2), d_x0 = umma_smem_desc(ring_addr + kXOff, 1024, 2);
-            const uint64_t d_b0 = umma_smem_desc(ring_addr, row_bytes * 8, lt), d_h0 = umma_smem_desc(ring_addr + kXOff, row_bytes * 8, lt);
-            uint32_t acc = tmem_base;
-            auto half_fp8 = [&](int slot, int h, uint32_t first) {        // one half of a k-block
-                const uint64_t off = (uint64_t)(uint32_t)(slot * (kSlot >> 4));
-                const uint64_t dx = d_x0 + off, dw = d_w0 + off + (uint64_t)(h * (kP2WBytes >> 4));
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    umma_f8f6f4_pair(acc + (uint32_t)(h * 256), dx + (uint64_t)(k * 2), dw + (uint64_t)(k * 2), idesc8, k > 0 ? 1u : first);
-            };
-            auto advance = [&](bool k_block) {
-                umma_commit_pair_at(empty_bar, 3);
-                ++it;
-                if (FP4) {
-                    sf_par = (sf_par >> 1) | (((sf_par & 1u) ^ (k_block ? 1u : 0u)) << (kStages - 1));
-                    dxl += kSlot >> 4;
-                    dwl += kSlot >> 4;
-                    sft += kSfCols;
-                    sf_bar += 8;
-                }
-                empty_bar += 8;
-                if (++st == kStages) {
-                    st = 0;
-                    ph ^= 1u;
-                    if (FP4) {
-                        dxl -= kStages * (kSlot >> 4);
-                        dwl -= kStages * (kSlot >> 4);
-                        sft -= kStages * kSfCols;
-                        sf_bar -= kStages * 8;
-                    }
-                    empty_bar -= kStages * 8;
-                }
-            };
-            auto k_block = [&](uint32_t first) -> bool {      // `first`: 0 for the tile's first (the accumulator starts there)
-                if (FP4) {
-                    // the scale copier saw both CTAs' operands land before it copied: one wait covers data and scales; the
-                    // barrier completes once per K-BLOCK use of the slot -- expand steps pass it by -- so it has its own parity
-                    if (!mbar_try_wait_at(sf_bar, sf_par & 1u) && !p2_wait<false>(p, ctrl, &ctrl->sf_ready[st], sf_par & 1u, limit_ns, 4, it)) return false;
-                    tc_fence_after();
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const uint32_t at = MX ? (uint32_t)k / 2u : (uint32_t)k;          // the atom that holds the MMA's scales
-                        const uint32_t ta = sft + at * 4u, tb = sft + 4u * kAtoms + at * 8u, acc_k = k > 0 ? 1u : first;
-                        if (!MX) umma_nvfp4_pair_lo<umma_idesc_nvfp4(256, 256)>(acc, dxl + k * 2, dwl + k * 2, ta, tb, acc_k);
-                        else if (k & 1) umma_mxfp4_pair_lo<umma_idesc_mxfp4(256, 256, 2)>(acc, dxl + k * 2, dwl + k * 2, ta, tb, acc_k);
-                        else umma_mxfp4_pair_lo<umma_idesc_mxfp4(256, 256, 0)>(acc, dxl + k * 2, dwl + k * 2, ta, tb, acc_k);
-                    }
-                } else {
-                    if (!p2_wait<true>(p, ctrl, &ctrl->full[st], ph, limit_ns, 4, it)) return false;
-#pragma unroll
-                    for (int h = 0; h < kHalves; ++h) half_fp8(st, h, first);
-                }
-                advance(true);
-                return true;
-            };
-            auto expand_step = [&]() -> bool {
-                if (!p2_wait<true>(p, ctrl, &ctrl->full[st], ph, limit_ns, 6, it)) return false;
-                if (STORED) {                                 // (completes once per EXPAND use of the slot: a parity of its own)
-                    if (!p2_wait<true>(p, ctrl, &ctrl->conv[st], (conv_par >> st) & 1u, limit_ns, 16, it)) return false;
-                    conv_par ^= 1u << st;
-                }
-                const uint64_t off = (uint64_t)(uint32_t)(st * (kSlot >> 4));
-                const uint64_t dh = d_h0 + off;
-#pragma unroll
-                for (int h = 0; h < kHalves; ++h) {
-                    const uint64_t db = d_b0 + off + (uint64_t)(h * (kP2WBytes >> 4));
-#pragma unroll
+            {   // (the role's body, on those under the names of what they hold)
+                uint8_t* const ring = ring_r;
+                P2Ctrl* const ctrl = ctrl_r;
+                const uint64_t limit_ns = limit_r;
+                const uint32_t tmem_base = tmem_r;
+                const int pair = pair_r, n_tiles = tiles_r, n_pairs = pairs_r, rc = rc_r;
+                // =========================================================== MMA issuer of the pair
+                // A = tokens (each CTA's 128 are its accumulator's lanes), B = features (128 from each CTA per 256-wide half)
+                const uint32_t idesc8 = umma_idesc(0, 0, 256, 256);
+                const uint32_t idesc16 = umma_idesc(1, 1, 256, 256);
+                const uint32_t row_bytes = (uint32_t)rc * 2;      // an expand tile's row: 32, 64 or 128 bytes, swizzled accordingly
+                const uint32_t lt = row_bytes == 128 ? 2u : row_bytes == 64 ? 4u : 6u;
+                int it = 0, st = 0;
+                uint32_t ph = 0, conv_par = 0;                    // phase of the slot; per slot: of its `conv` barrier
+                const uint32_t ring_addr = smem_u32(ring);
+                // NVFP4, MXFP4: what a slot's MMAs need as running values -- the loop's thread issues four MMAs of 128 cycles each per slot and
+                // its own 70 or so instructions must not take longer
+                uint32_t sf_par = 0;                              // phases of the scale barriers, the slot's own in bit 0
+                uint32_t dxl = (uint32_t)umma_smem_desc(ring_addr + kXOff, 1024, 2), dwl = (uint32_t)umma_smem_desc(ring_addr, 1024, 2);
+                uint32_t sft = tmem_base + 256u, sf_bar = smem_u32(ctrl->sf_ready), empty_bar = smem_u32(ctrl->empty);
+                const uint64_t d_w0 = umma_smem_desc(ring_addr, 1024, 2), d_x0 = umma_smem_desc(ring_addr + kXOff, 1024, 2);
+                const uint64_t d_b0 = umma_smem_desc(ring_addr, row_bytes * 8, lt), d_h0 = umma_smem_desc(ring_addr + kXOff, row_bytes * 8, lt);
+                uint32_t acc = tmem_base;
+                auto half_fp8 = [&](int slot, int h, uint32_t first) {        // one half of a k-block
+                    const uint64_t off = (uint64_t)(uint32_t)(slot * (kSlot >> 4));
+                    const uint64_t dx = d_x0 + off, dw = d_w0 + off + (uint64_t)(h * (kP2WBytes >> 4));
+    #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        if (k * 16 < rc)
-                            umma_f16_pair(acc + (uint32_t)(h * 256), dh + (uint64_t)(k * 2), db + (uint64_t)(k * 2), idesc16, 1u);
-                }
-                advance(false);
-                return true;
-            };
-            bool ok = true;
-            for (int t = pair, i = 0; t < n_tiles && ok; t += n_pairs, ++i) {
-                acc = tmem_base + (uint32_t)(i % kAccBufs) * 256u;
-                const int use = kHalves == 2 ? i : i / kAccBufs;          // the epilogues have read the accumulator's previous tile
-                if (use > 0) {
-                    if (!p2_wait<true>(p, ctrl, &ctrl->acc_empty[kHalves == 2 ? 0 : i % kAccBufs], (uint32_t)((use - 1) & 1), limit_ns, 8, i)) break;
-                    tc_fence_after();
-                }
-                int kb = 0;
-                if (kHalves == 2) {
-                    // The halves of the accumulator come free one after the other: the first ring's worth of k-blocks goes into the
-                    // first half while the epilogues still read the second, then into the second.
-                    const int n = min(kStages, kblocks);
-                    int s2 = st;
-                    uint32_t ph2 = ph;
-                    for (int j = 0; j < n && ok; ++j) {
-                        ok = p2_wait<true>(p, ctrl, &ctrl->full[s2], ph2, limit_ns, 4, it + j);
-                        if (ok) half_fp8(s2, 0, j > 0 ? 1u : 0u);
-                        if (++s2 == kStages) { s2 = 0; ph2 ^= 1u; }
+                        umma_f8f6f4_pair(acc + (uint32_t)(h * 256), dx + (uint64_t)(k * 2), dw + (uint64_t)(k * 2), idesc8, k > 0 ? 1u : first);
+                };
+                auto advance = [&](bool k_block) {
+                    umma_commit_pair_at(empty_bar, 3);
+                    ++it;
+                    if (FP4) {
+                        sf_par = (sf_par >> 1) | (((sf_par & 1u) ^ (k_block ? 1u : 0u)) << (kStages - 1));
+                        dxl += kSlot >> 4;
+                        dwl += kSlot >> 4;
+                        sft += kSfCols;
+                        sf_bar += 8;
                     }
-                    if (ok && use > 0) {
-                        ok = p2_wait<true>(p, ctrl, &ctrl->acc_empty[1], (uint32_t)((use - 1) & 1), limit_ns, 8, i);
+                    empty_bar += 8;
+                    if (++st == kStages) {
+                        st = 0;
+                        ph ^= 1u;
+                        if (FP4) {
+                            dxl -= kStages * (kSlot >> 4);
+                            dwl -= kStages * (kSlot >> 4);
+                            sft -= kStages * kSfCols;
+                            sf_bar -= kStages * 8;
+                        }
+                        empty_bar -= kStages * 8;
+                    }
+                };
+                auto k_block = [&](uint32_t first) -> bool {      // `first`: 0 for the tile's first (the accumulator starts there)
+                    if (FP4) {
+                        // the scale copier saw both CTAs' operands land before it copied: one wait covers data and scales; the
+                        // barrier completes once per K-BLOCK use of the slot -- expand steps pass it by -- so it has its own parity
+                        if (!mbar_try_wait_at(sf_bar, sf_par & 1u) && !p2_wait<false>(p, ctrl, &ctrl->sf_ready[st], sf_par & 1u, limit_ns, 4, it)) return false;
+                        tc_fence_after();
+    #pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t at = MX ? (uint32_t)k / 2u : (uint32_t)k;          // the atom that holds the MMA's scales
+                            const uint32_t ta = sft + at * 4u, tb = sft + 4u * kAtoms + at * 8u, acc_k = k > 0 ? 1u : first;
+                            if (!MX) umma_nvfp4_pair_lo<umma_idesc_nvfp4(256, 256)>(acc, dxl + k * 2, dwl + k * 2, ta, tb, acc_k);
+                            else if (k & 1) umma_mxfp4_pair_lo<umma_idesc_mxfp4(256, 256, 2)>(acc, dxl + k * 2, dwl + k * 2, ta, tb, acc_k);
+                            else umma_mxfp4_pair_lo<umma_idesc_mxfp4(256, 256, 0)>(acc, dxl + k * 2, dwl + k * 2, ta, tb, acc_k);
+                        }
+                    } else {
+                        if (!p2_wait<true>(p, ctrl, &ctrl->full[st], ph, limit_ns, 4, it)) return false;
+    #pragma unroll
+                        for (int h = 0; h < kHalves; ++h) half_fp8(st, h, first);
+                    }
+                    advance(true);
+                    return true;
+                };
+                auto expand_step = [&]() -> bool {
+                    if (!p2_wait<true>(p, ctrl, &ctrl->full[st], ph, limit_ns, 6, it)) return false;
+                    if (STORED) {                                 // (completes once per EXPAND use of the slot: a parity of its own)
+                        if (!p2_wait<true>(p, ctrl, &ctrl->conv[st], (conv_par >> st) & 1u, limit_ns, 16, it)) return false;
+                        conv_par ^= 1u << st;
+                    }
+                    const uint64_t off = (uint64_t)(uint32_t)(st * (kSlot >> 4));
+                    const uint64_t dh = d_h0 + off;
+    #pragma unroll
+                    for (int h = 0; h < kHalves; ++h) {
+                        const uint64_t db = d_b0 + off + (uint64_t)(h * (kP2WBytes >> 4));
+    #pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (k * 16 < rc)
+                                umma_f16_pair(acc + (uint32_t)(h * 256), dh + (uint64_t)(k * 2), db + (uint64_t)(k * 2), idesc16, 1u);
+                    }
+                    advance(false);
+                    return true;
+                };
+                bool ok = true;
+                for (int t = pair, i = 0; t < n_tiles && ok; t += n_pairs, ++i) {
+                    acc = tmem_base + (uint32_t)(i % kAccBufs) * 256u;
+                    const int use = kHalves == 2 ? i : i / kAccBufs;          // the epilogues have read the accumulator's previous tile
+                    if (use > 0) {
+                        if (!p2_wait<true>(p, ctrl, &ctrl->acc_empty[kHalves == 2 ? 0 : i % kAccBufs], (uint32_t)((use - 1) & 1), limit_ns, 8, i)) break;
                         tc_fence_after();
                     }
-                    if (!ok) break;
-                    for (; kb < n; ++kb) {
-                        half_fp8(st, 1, kb > 0 ? 1u : 0u);
-                        advance(true);
+                    int kb = 0;
+                    if (kHalves == 2) {
+                        // The halves of the accumulator come free one after the other: the first ring's worth of k-blocks goes into the
+                        // first half while the epilogues still read the second, then into the second.
+                        const int n = min(kStages, kblocks);
+                        int s2 = st;
+                        uint32_t ph2 = ph;
+                        for (int j = 0; j < n && ok; ++j) {
+                            ok = p2_wait<true>(p, ctrl, &ctrl->full[s2], ph2, limit_ns, 4, it + j);
+                            if (ok) half_fp8(s2, 0, j > 0 ? 1u : 0u);
+                            if (++s2 == kStages) { s2 = 0; ph2 ^= 1u; }
+                        }
+                        if (ok && use > 0) {
+                            ok = p2_wait<true>(p, ctrl, &ctrl->acc_empty[1], (uint32_t)((use - 1) & 1), limit_ns, 8, i);
+                            tc_fence_after();
+                        }
+                        if (!ok) break;
+                        for (; kb < n; ++kb) {
+                            half_fp8(st, 1, kb > 0 ? 1u : 0u);
+                            advance(true);
+                        }
                     }
+                    const int lead = STORED ? min(kStages, kblocks) : kblocks;
+                    for (; kb < lead && ok; ++kb) ok = k_block(kb > 0 ? 1u : 0u);
+                    if (!ok || !p2_wait<false>(p, ctrl, &ctrl->meta_full[i & 1], (uint32_t)((i >> 1) & 1), limit_ns, 5, it)) { ok = false; break; }
+                    const int n_steps = ctrl->meta[i & 1].n_steps;
+                    if (STORED) {
+                        P2Walk walk(lead, kblocks, n_steps);
+                        for (int q = 0; q < walk.rem && ok; ++q) ok = walk.next_is_step() ? expand_step() : k_block(1u);
+                    } else {
+                        for (int li = 0; li < n_steps && ok; ++li) ok = expand_step();
+                    }
+                    if (ok) umma_commit_pair(&ctrl->acc_full[i % kAccBufs], 3);
                 }
-                const int lead = STORED ? min(kStages, kblocks) : kblocks;
-                for (; kb < lead && ok; ++kb) ok = k_block(kb > 0 ? 1u : 0u);
-                if (!ok || !p2_wait<false>(p, ctrl, &ctrl->meta_full[i & 1], (uint32_t)((i >> 1) & 1), limit_ns, 5, it)) { ok = false; break; }
-                const int n_steps = ctrl->meta[i & 1].n_steps;
-                if (STORED) {
-                    P2Walk walk(lead, kblocks, n_steps);
-                    for (int q = 0; q < walk.rem && ok; ++q) ok = walk.next_is_step() ? expand_step() : k_block(1u);
-                } else {
-                    for (int li = 0; li < n_steps && ok; ++li) ok = expand_step();
-                }
-                if (ok) umma_commit_pair(&ctrl->acc_full[i % kAccBufs], 3);
-            }
             }
         }
         if (STORED && lane == 0 && rank == 1) {
@@ -533,8 +533,8 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
         }
     } else if (FP4 && warp == 14) {
         // =========================================================== TMA producer of the block scales (NVFP4, MXFP4): a thread of its own,
-        // because a copy costs its issuer some 130 cycles and five of them per slot bounded the main loop at 780 cycles, whose four MMAs
-        // take 513.  The bytes count on the same barrier, whose phase is rank 0's warp 0's to open.
+        // because a copy costs its issuer some 130 cycles, and five of them per slot, with the slot's wait and announcement, bounded the main
+        // loop at 780 cycles, whose four MMAs take 513.  The bytes count on the same barrier, whose phase is rank 0's warp 0's to open.
         if (lane == 0) {
             griddep_wait();
             int st = 0, it = 0, steps = 0, last_step = -kStages - 1;      // expand steps so far, the slot count at the last of them
@@ -582,7 +582,7 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
         // =========================================================== scale copiers (NVFP4, MXFP4, rank 0; warps 3, 12, 13): a k-block
         // slot's scale factors -> both CTAs' tensor memory, ahead of the MMAs.  Threads of their own because every tcgen05
         // instruction costs its issuer some 50 cycles: twelve copies per slot from one thread (with its wait and commit, 920
-        // cycles) bounded the main loop, whose four MMAs take the tensor pipe some 540.  Copier 0 moves the tokens' scales,
+        // cycles) bounded the main loop, whose four MMAs take the tensor pipe 513.  Copier 0 moves the tokens' scales,
         // copiers 1 and 2 those of the two 128-feature halves of W: four copies (MXFP4: two) each per slot.
         const int cpi = warp == 3 ? 0 : warp - 11;
         if (FP4 && lane == 0 && rank == 0 && cpi < 3) {

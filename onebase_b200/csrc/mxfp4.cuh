@@ -12,8 +12,6 @@
 
 namespace ob {
 
-constexpr int kMxBlock = 32;
-
 // Bits of |v|: as integers they order like the magnitudes, infinity above every number and NaN above infinity.
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 

@@ -309,7 +309,7 @@ int resident_clusters(const ObLayerDesc& d, int split2, size_t smem) {
 // of up to 32 tokens; for an MXFP4 base of 64 too where the table, R up to 64, lets two CTAs share an SM: 64 tokens, us, per step -> table:
 // gate_up, 32 tenants of rank 64 90 -> 76, 16 NVFP4-stored ones 96 -> 70; split two ways qkv, 16 of rank 32 33 -> 28, 16 FP8-stored of rank 64
 // 52 -> 38; four ways o, 32 of rank 16 29 -> 24, down, 16 of rank 64 38.3 -> 34.6, 8 30.7 -> 31.6.  (K1's splits as they were then.)
-bool k2_decode_form(const ObLayerDesc& d, int tn, int split2, int mma_shrink) {
+bool k2_decode_form(const ObLayerDesc& d, int tn, int mma_shrink) {
     return tn <= kDecodeTokens || (d.base_fmt == OB_BASE_MXFP4 && tn == 64 && d.R <= 64 && !mma_shrink);
 }
 
@@ -424,16 +424,15 @@ int resolve_cfg(const ObLayer* l, int M, const ObTileCfg* cfg, Resolved* r, int 
     // 34.6 -> 24.7; tp8_gate_up, one token 19.2 -> 17.0 (5 -> 4; 2, which would be clusters, 17.9); 64 tokens, 32 FP8-stored of rank 64,
     // 2 -> 4: qkv 41.6 -> 39.1, tp4_gate_up 50.5 -> 45.4.
     if (d.base_fmt == OB_BASE_MXFP4 && r->m_tiles == 1 && r->tn <= 64 && !(cfg && cfg->split2)) {
+        const int form = k2_decode_form(d, r->tn, r->mma_shrink) ? 1 : 0;
+        const int ring = ring_stages(d, r->tn, l->rc, form, cfg && cfg->stages ? cfg->stages : 0);
+        const size_t smem = ring > 0 ? k2_fp8_smem_bytes(r->tn, ring, l->rc, d.R, d.base_fmt, form) : 0;
         r->split2 = 1;
-        for (const int c : {8, 4, 2}) {
-            const int form = k2_decode_form(d, r->tn, c, r->mma_shrink) ? 1 : 0;
-            const int ring = ring_stages(d, r->tn, l->rc, form, cfg && cfg->stages ? cfg->stages : 0);
-            if (ring > 0 && l->n_tiles * c <= 296 && kblocks / c >= 4 &&
-                l->n_tiles <= resident_clusters(d, c, k2_fp8_smem_bytes(r->tn, ring, l->rc, d.R, d.base_fmt, form))) {
+        for (const int c : {8, 4, 2})
+            if (ring > 0 && l->n_tiles * c <= 296 && kblocks / c >= 4 && l->n_tiles <= resident_clusters(d, c, smem)) {
                 r->split2 = c;
                 break;
             }
-        }
         const int twice = r->split2 * 2;
         if (l->n_tiles * twice <= 296 && twice <= 8 &&
             ((M <= kDecodeTokens && kblocks > 6 * twice) || (M > kDecodeTokens && (d.R > 64 || d.lora_fmt != kLoraBf16) && twice == 4 && kblocks >= 4 * twice)))
@@ -465,7 +464,7 @@ int resolve_cfg(const ObLayer* l, int M, const ObTileCfg* cfg, Resolved* r, int 
             // 128, 1 -> 2 splits, 2208 warps: 31.4 -> 25.4; qkv, 32 of rank 64, FP8-stored, 2 -> 4, some 3000 warps: 25.8 -> 26.8); for more, two
             // waves (64 tokens, 32 tenants of rank 64, one -> two: down 40.9 -> 34.5, tp4_gate_up 63.0 -> 49.9), unless many feature tiles
             // each sum the partials for every step (gate_up, 16 of rank 128, 1 -> 2 splits: 79.6 -> 94.7).
-            const long long most = M <= kDecodeTokens || (l->n_tiles > 100 && !k2_decode_form(d, r->tn, r->split2, 0)) ? 2400 : 4096;
+            const long long most = M <= kDecodeTokens || (l->n_tiles > 100 && !k2_decode_form(d, r->tn, 0)) ? 2400 : 4096;
             while (split1 < 16 && d.K / (split1 * 2) >= 900 && units * split1 * 2 <= most) split1 *= 2;
         }
         else if (pb == 1)   // decode: as many K splits as keep the whole shrink in one wave of the GPU's 2 x 148 CTA slots (8 warps each)
@@ -485,7 +484,7 @@ int resolve_cfg(const ObLayer* l, int M, const ObTileCfg* cfg, Resolved* r, int 
         while (r->split1 > 1 && (long long)(r->split1 - 1) * r->k_per_split >= d.K) --r->split1;
     r->pb = pb;
     const int rc = l->rc;
-    const int small = k2_decode_form(d, r->tn, r->split2, r->mma_shrink) ? 1 : 0;
+    const int small = k2_decode_form(d, r->tn, r->mma_shrink) ? 1 : 0;
     int stages = r->stream ? r->stages : (cfg && cfg->stages) ? cfg->stages : 0;
     if (r->stream) {
         r->wait_ms = (cfg && cfg->wait_ms > 0) ? (uint32_t)cfg->wait_ms : 2000u;
@@ -674,7 +673,7 @@ int k2_prepare(ObLayer* l, const ObBatch* b, void* ws, const ObWorkspaceShape* s
     p.stages = r.stages;
     p.rc = l->rc;
     p.nh = k2_fp8_h_tiles(r.tn);
-    p.small = k2_decode_form(d, r.tn, r.split2, r.mma_shrink) ? 1 : 0;
+    p.small = k2_decode_form(d, r.tn, r.mma_shrink) ? 1 : 0;
     p.wsf = static_cast<const uint8_t*>(d.w_sf);
     p.xsf = base + lay.xsf;
     p.alpha = d.alpha;

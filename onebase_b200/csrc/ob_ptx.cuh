@@ -383,28 +383,8 @@ __device__ __forceinline__ void umma_f8f6f4_pair(uint32_t d_tmem, uint64_t a_des
         "}\n" ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-__device__ __forceinline__ void umma_nvfp4_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa_tmem,
-                                                uint32_t sfb_tmem, uint32_t accumulate) {
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "setp.ne.b32 p, %6, 0;\n"
-        "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n"
-        "}\n" ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
-        : "memory");
-}
-__device__ __forceinline__ void umma_mxfp4_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa_tmem,
-                                                uint32_t sfb_tmem, uint32_t accumulate) {
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "setp.ne.b32 p, %6, 0;\n"
-        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n"
-        "}\n" ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
-        : "memory");
-}
-// The same two MMAs for a loop whose issuing thread is what bounds it: descriptors by their low words (the high word is the same for
-// every operand of the kind), everything else known at compile time.
+// The block-scaled MMAs of a pair, for a loop whose issuing thread is what bounds it: descriptors by their low words (the high word is the
+// same for every operand of the kind), everything else known at compile time.
 constexpr uint32_t kUmmaDescHigh128 = (1024u >> 4) | (1u << 14) | (2u << 29);      // of umma_smem_desc(.., 1024, 2)
 template <uint32_t IDESC>
 __device__ __forceinline__ void umma_mxfp4_pair_lo(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t sfa_tmem, uint32_t sfb_tmem,

@@ -91,9 +91,11 @@ __device__ __forceinline__ void norm_reduce(float& sum, float& top) {
 }
 __device__ __forceinline__ float norm_rstd(float sum, const ObRmsNorm& p) { return __frcp_rn(__fsqrt_rn(__fdiv_rn(sum, (float)p.K) + p.eps)); }
 
-// Any row, element by element: G threads, NE elements each held in registers (NE = 0: the row is read twice instead).
+// Any row, element by element: G threads, NE elements each held in registers (NE = 0: the row is read twice instead).  Eight elements
+// each: bound to the 32 registers that let an SM have its 2048 threads, at a spill of 8 bytes (with 34 and the bound, us: 2048 rows of 7393 --
+// one CTA of 1024 threads per SM -- 89 -> 57, 4096 of 4001 64 -> 54, 8192 of 1999 59 -> 52, 8192 of 777 24 -> 22, but 300 of 4001 6.8 -> 7.5).
 template <typename T, int G, int NE>
-__global__ void __launch_bounds__(norm_block(G)) rms_norm_any_kernel(const ObRmsNorm p) {
+__global__ void __launch_bounds__(norm_block(G), NE == 8 && G >= 128 ? 2048 / G : 0) rms_norm_any_kernel(const ObRmsNorm p) {
     constexpr int kRows = norm_block(G) / G;
     const int t = threadIdx.x % G, lane = threadIdx.x & 31;
     const long long row = (long long)blockIdx.x * kRows + threadIdx.x / G;
@@ -163,7 +165,7 @@ __global__ void __launch_bounds__(norm_block(G)) rms_norm_any_kernel(const ObRms
 }
 
 // Rows that take 16-byte accesses: G threads hold one row in registers, NV groups of eight elements each, so that every tensor crosses
-// memory once (bound by memory: 9 bytes per element with residual and FP8 codes, 8192 rows of 4096 at 6.3 TB/s).  Up to 32 threads a
+// memory once (bound by memory: 9 bytes per element with residual and FP8 codes, 8192 rows of 4096 in 51 us, 5.9 TB/s).  Up to 32 threads a
 // row is a part of one warp and needs no barrier; above, one.  The new residual stream is stored as soon as it is formed and only
 // s w is kept across the reduction.
 template <typename T>
@@ -333,8 +335,9 @@ static cudaError_t launch_typed(const ObRmsNorm& p, cudaStream_t stream) {
     const bool rows = p.K % 8 == 0 && p.K <= 32768 && whole(p.x, p.x_ld, p.x_hd) && whole(p.residual, p.residual_ld, p.residual_hd) &&
                       whole(p.residual_out, p.residual_out_ld, p.residual_out_hd) && whole(p.y, p.y_ld, p.y_hd) && whole(p.weight, 0, 0);
     if (!rows) {
-        // eight elements per thread where they suffice: 2048 rows of 7393 59 us (256 threads reading the row twice 74), 4096 of 4001 61
-        // (73), 8192 of 777 27 (42), 16 of 7393 5.6 (18)
+        // eight elements per thread where they suffice: 2048 rows of 7393 57 us (256 threads reading the row twice 74), 4096 of 4001 54
+        // (73), 8192 of 777 22 (42), 16 of 7393 5.1 (18).  Two bytes per access: the rows begin anywhere, and vectors would need a head and a
+        // tail of their own for every tensor
         if (p.K <= 128) return launch_any<T, 32, 4>(p, stream);
         if (p.K <= 256) return launch_any<T, 32, 8>(p, stream);
         if (p.K <= 512) return launch_any<T, 64, 8>(p, stream);

@@ -90,13 +90,18 @@ struct P2Ctrl {
     uint64_t conv[kP2MaxStages];     // stored adapters: this CTA's B tiles of the expand step are in the slot (its 8 epilogue warps) ...
                                      // ... and, rank 0's, the partner's are (its relay's arrival)
     uint64_t empty[kP2MaxStages];    // the pair's MMAs on the slot are done (arrives in both CTAs)
+    // NVFP4, MXFP4: this CTA's producer has acquired the slot for a k-block.  The block scales' producer and the scale copiers put nothing into
+    // an expand step's slot, so nothing holds the ring back for them there: one that followed such a slot's barriers and came two phases
+    // late would take the phase in progress for the awaited one and wait for good.  They pass steps by and wait here, where a phase is a
+    // k-block's use of the slot and the next one needs their own part in this.
+    uint64_t k_free[kP2MaxStages];
     uint64_t meta_full[2];
     uint64_t meta_empty[2];
     uint64_t acc_full[2];            // per accumulator buffer; arrives in both CTAs
     uint64_t acc_empty[2];           // rank 0 only: both CTAs' epilogue warps (16 arrivals)
     uint32_t tmem_base;
     volatile int abort_flag;
-    volatile int b_grant;            // expand steps whose slot the producer has acquired (stored adapters: for the epilogue warps to fill)
+    volatile int b_grant;            // stored adapters: expand steps whose slot the producer has acquired for the epilogue warps to fill
     int go_flag;
     P2Meta meta[2];
 };
@@ -128,24 +133,6 @@ __device__ __forceinline__ bool p2_wait(const K2pParams& p, P2Ctrl* c, uint64_t*
             }
         }
     }
-}
-
-// The scale copiers and the scales' producer put nothing into an expand step's slot, so nothing holds the ring back for them there: one
-// that waited on such a slot's barriers and came two phases late would take the phase in progress for the awaited one and wait for
-// good.  They pass steps by, and before they wait on a k-block's slot again they see by this count, which cannot be mistaken, that the
-// producer has acquired the slots of all `steps` expand steps in front of it: the slot's earlier uses are then over but for the last, and its
-// next one needs their own part, so the slot's free barrier is in the awaited phase or the one behind it.
-__device__ __forceinline__ bool p2_granted(const K2pParams& p, P2Ctrl* c, int steps, uint64_t limit_ns, int where, int it) {
-    if (c->b_grant >= steps) return true;
-    const uint64_t t0 = global_timer_ns();
-    for (uint32_t n = 1; c->b_grant < steps; ++n) {
-        if (c->abort_flag) return false;
-        if ((n & 63u) == 0 && global_timer_ns() - t0 > limit_ns) {
-            p2_timeout(p, c, where, it);
-            return false;
-        }
-    }
-    return true;
 }
 
 // The value in a register of its own from here on.  The epilogue's registers push what the whole kernel uses into local memory, and a
@@ -258,6 +245,7 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
             mbar_init(&ctrl->sf_ready[i], 3);   // one commit per copier thread
             mbar_init(&ctrl->conv[i], rank == 0 ? 9 : 8);
             mbar_init(&ctrl->empty[i], 1);
+            mbar_init(&ctrl->k_free[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&ctrl->meta_full[i], 1);
@@ -326,6 +314,7 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
                     // between the partner's data and the MMAs
                     const uint32_t bar0 = cluster_peer_addr(smem_u32(&ctrl->full[st]), 0);
                     if (!step) {
+                        if (FP4) mbar_arrive(&ctrl->k_free[st]);
                         if (rank == 0) mbar_arrive_expect_tx(&ctrl->full[st], (uint32_t)(2 * kSlot));
 #pragma unroll
                         for (int h = 0; h < kHalves; ++h)
@@ -341,7 +330,7 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
                         const bool in = entry != kP2NoEntry;
                         const int h_row = in ? tl.s * p.max_m + tl.t0 + (int)rank * 128 : p.S * p.max_m + 128;
                         const int h_col = in ? entry * p.R + (int)e.chunk * rc : 0;
-                        if (STORED || FP4) {                  // the slot is free: the epilogue warps fill its B tiles; p2_granted counts it
+                        if (STORED) {                         // the slot is free: the epilogue warps fill its B tiles
                             __threadfence_block();
                             ctrl->b_grant = ++granted;
                         }
@@ -537,8 +526,8 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
         // loop at 780 cycles, whose four MMAs take 513.  The bytes count on the same barrier, whose phase is rank 0's warp 0's to open.
         if (lane == 0) {
             griddep_wait();
-            int st = 0, it = 0, steps = 0, last_step = -kStages - 1;      // expand steps so far, the slot count at the last of them
-            uint32_t ph = 1;
+            int st = 0, it = 0;
+            uint32_t k_par = 0;                               // phases of the slots' `k_free` barriers
             bool ok = true;
             for (int t = pair, i = 0; t < n_tiles && ok; t += n_pairs, ++i) {
                 const P2Tile tl = p2_tile(p, t, m_tiles, kRows);
@@ -556,15 +545,12 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
                         total += walk.n_steps;
                     }
                     if (q >= lead) step = walk.next_is_step();
-                    if (step) {
-                        ++steps;
-                        last_step = it;
-                    } else {
-                        if ((it - last_step <= kStages && !p2_granted(p, ctrl, steps, limit_ns, 22, it)) ||
-                            !p2_wait<true>(p, ctrl, &ctrl->empty[st], ph, limit_ns, 21, it)) {
+                    if (!step) {
+                        if (!p2_wait<false>(p, ctrl, &ctrl->k_free[st], (k_par >> st) & 1u, limit_ns, 21, it)) {
                             ok = false;
                             break;
                         }
+                        k_par ^= 1u << st;
                         // as 8 (MXFP4: 4) x 256-byte rows of a [rows, 256] byte tensor: this CTA's 128 tokens (the MMA's A rows), then both
                         // 128-feature tiles of W (every CTA needs the scales of all of B's 256 rows in its own tensor memory)
                         const uint32_t bar0 = cluster_peer_addr(smem_u32(&ctrl->full[st]), 0);
@@ -574,7 +560,7 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
                         tma_load_2d_pair(sf + 2 * kSf, &tm_wsf, bar0, 0, ((tl.sf_tile + 1) * p.kblocks + kb) * (kSf / 256));
                         ++kb;
                     }
-                    if (++st == kStages) { st = 0; ph ^= 1u; }
+                    if (++st == kStages) st = 0;
                 }
             }
         }
@@ -586,8 +572,8 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
         // copiers 1 and 2 those of the two 128-feature halves of W: four copies (MXFP4: two) each per slot.
         const int cpi = warp == 3 ? 0 : warp - 11;
         if (FP4 && lane == 0 && rank == 0 && cpi < 3) {
-            int it = 0, st = 0, steps = 0, last_step = -kStages - 1;      // (as the scales' producer's)
-            uint32_t ph = 0;
+            int it = 0, st = 0, last_step = -kStages - 1;
+            uint32_t ph = 0, k_par = 0;
             bool ok = true;
             for (int t = pair, i = 0; t < n_tiles && ok; t += n_pairs, ++i) {
                 // the tile's expand steps use ring slots too: read their number now (the scout is a tile ahead), while this
@@ -602,17 +588,16 @@ k2_prefill_pair_kernel(const K2pParams p, const __grid_constant__ CUtensorMap tm
                 for (int q = 0; q < total; ++q, ++it) {
                     const bool step = q >= lead && walk.next_is_step();
                     if (step) {
-                        ++steps;
                         last_step = it;
                     } else {
-                        // behind expand steps: once the slot's last use is over, its full barrier is in this use's phase (a parity wait
-                        // entered a whole phase early would pass at once)
-                        if ((it - last_step <= kStages && (!p2_granted(p, ctrl, steps, limit_ns, 23, it) ||
-                                                           !p2_wait<true>(p, ctrl, &ctrl->empty[st], ph ^ 1u, limit_ns, 24, it))) ||
+                        // behind expand steps: once the slot is acquired for this use, its last use is over and its full barrier in this
+                        // use's phase (a parity wait entered a whole phase early would pass at once)
+                        if ((it - last_step <= kStages && !p2_wait<false>(p, ctrl, &ctrl->k_free[st], (k_par >> st) & 1u, limit_ns, 22, it)) ||
                             !p2_wait<true>(p, ctrl, &ctrl->full[st], ph, limit_ns, 13, it)) {
                             ok = false;
                             break;
                         }
+                        k_par ^= 1u << st;
                         tc_fence_after();
                         const uint32_t sfs = smem_u32(ring + (size_t)st * kSlot) + (uint32_t)(kXOff + kP2XBytes);
                         const uint32_t sft = tmem_base + 256u + (uint32_t)(st * kSfCols);

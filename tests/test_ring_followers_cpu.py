@@ -14,11 +14,11 @@ STAGES = 5
 
 
 def passes_steps_by(where: int) -> bool:
-    """Whether the loop whose slot wait is numbered `where` waits only in k-block slots, behind p2_granted."""
+    """Whether the loop whose slot wait is numbered `where` waits only in k-block slots, behind the producer's `k_free`."""
     text = SOURCE.read_text()
     at = text.index(f"limit_ns, {where}, it)")
     body = text[text.rindex("for (int q = 0", 0, at): at]
-    return re.search(r"if \(step\) \{\s*\+\+steps;\s*last_step = it;\s*\} else \{", body) is not None and "p2_granted(" in body
+    return re.search(r"if \(!step\) \{|if \(step\) \{\s*last_step = it;\s*\} else \{", body) is not None and "&ctrl->k_free[st]" in body
 
 
 class Barrier:
@@ -40,38 +40,44 @@ class Barrier:
 
 def ring(tiles, by_scales: bool, by_copier: bool):
     """Generators of the roles; each yields a predicate to wait for.  `tiles`: per tile the slots, True = expand step."""
-    full, sf, empty = ([Barrier() for _ in range(STAGES)] for _ in range(3))
-    grant = [0]
+    full, sf, empty, k_free = ([Barrier() for _ in range(STAGES)] for _ in range(4))
     slots = [step for t in tiles for step in t]
 
     def producer():
-        steps = 0
         for it, step in enumerate(slots):
             st, ph = it % STAGES, (it // STAGES + 1) & 1
             yield lambda: empty[st].passed(ph)
-            if step:
-                steps += 1
-                grant[0] = steps
+            if not step:
+                k_free[st].arrive("producer", {"producer"})
             full[st].arrive("data", {"data"} if step else {"data", "scales"})
 
-    def follower(by: bool, wait_empty_first: bool, act):
-        steps, last = 0, -STAGES - 1
+    def scales(by: bool):
+        uses = [0] * STAGES
         for it, step in enumerate(slots):
             st, use = it % STAGES, it // STAGES
-            free, ready = (use + 1) & 1, use & 1
+            if not by:
+                yield lambda: empty[st].passed((use + 1) & 1)
+            elif not step:
+                yield lambda: k_free[st].passed(uses[st] & 1)
+                uses[st] += 1
+            if not step:
+                give_scales(st, use)
+
+    def copier(by: bool):
+        uses, last = [0] * STAGES, -STAGES - 1
+        for it, step in enumerate(slots):
+            st, use = it % STAGES, it // STAGES
             if step:
-                steps, last = steps + 1, it
+                last = it
                 if by:
                     continue
-            elif by and it - last <= STAGES:
-                yield lambda: grant[0] >= steps
-                yield lambda: empty[st].passed(free)
-            if wait_empty_first:
-                yield lambda: empty[st].passed(free)
-            else:
-                yield lambda: full[st].passed(ready)
+            elif by:
+                if it - last <= STAGES:
+                    yield lambda: k_free[st].passed(uses[st] & 1)
+                uses[st] += 1
+            yield lambda: full[st].passed(use & 1)
             if not step:
-                act(st, use)
+                copy(st, use)
 
     def give_scales(st, use):
         assert empty[st].done >= use, "scales into a slot that is not free"
@@ -92,8 +98,7 @@ def ring(tiles, by_scales: bool, by_copier: bool):
                 seen[st] += 1
             empty[st].arrive("mma", {"mma"})
 
-    return {"producer": producer(), "scales": follower(by_scales, True, give_scales), "copier": follower(by_copier, False, copy),
-            "issuer": issuer()}
+    return {"producer": producer(), "scales": scales(by_scales), "copier": copier(by_copier), "issuer": issuer()}
 
 
 def finishes(tiles, late: str, by_scales: bool, by_copier: bool) -> bool:

@@ -34,8 +34,8 @@
 // reason); warp 1 = in the pair's rank-0 CTA the MMA issuer for both; warp 2 = tile
 // scout (row map, output scale, expand steps; both CTAs compute the same list); warps 4..11 = epilogue of the CTA's own
 // 128 tokens (straight from tensor memory to y; two warps per lane quarter, half of the features each);
-// warps 3, 12, 13 = in rank 0 the scale copiers (tcgen05.cp of a slot's scale factors into both CTAs' tensor memory).  The
-// epilogue's two warpgroups take registers from the other two, so that a warp can hold 128 features of its tokens as bf16 and
+// warps 3, 12, 13 = in rank 0 the scale copiers (tcgen05.cp of a slot's scale factors into both CTAs' tensor memory); warp 14 = TMA
+// producer of the block scales.  The epilogue's two warpgroups take registers from the other two, so that a warp can hold 128 features of its tokens as bf16 and
 // the accumulator is free after eight loads; 512-feature tiles are read out, and started, one 256-feature half after the other.
 // (8192 tokens of gate_up: from the accumulator's last MMA to the next tile's first 3.5 -> 0.8 us, the call 822 -> 790.)  The
 // issuer's commits arrive on the slot-free and accumulator-full barriers of BOTH CTAs (tcgen05.commit ... multicast::cluster, an arrival, not a load).  The kernel is persistent: a pair walks the launch's

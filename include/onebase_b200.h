@@ -249,10 +249,10 @@ int ob_k2_fp8_static(ObLayer* layer, const ObBatch* batch, void* workspace, cons
 int ob_chain_fp8(ObLayer* layer, const ObBatch* batch, void* workspace, const ObWorkspaceShape* shape,
                  const ObTileCfg* cfg, void* cuda_stream);
 
-/* A projection's kernels start beside the launch before them in the stream and read weights, scales and adapters before they wait for
- * it.  So that launch must not be the one that writes them: behind a kernel or copy that (re)writes an operand in place, and directly in
- * front of the next projection, call this (one empty launch; capturable).  Any launch without the programmatic attribute in between does as
- * well.  ob_*_pack_scales and ob_requant_* end with it; ob_mxfp4_quantize and ob_mxfp4_dequantize, whose outputs are activations as often, do
+/* A projection's kernels start beside the launch before them in the stream and read weights, scales, adapters and the batch's index (tok ..
+ * seg_ids) before they wait for it.  So that launch must not be the one that writes them: behind a kernel or copy that (re)writes one of them,
+ * and directly in front of the next projection, call this (one empty launch; capturable).  Any launch or copy without the programmatic
+ * attribute in between does as well.  ob_*_pack_scales and ob_requant_* end with it; ob_mxfp4_quantize and ob_mxfp4_dequantize, whose outputs are activations as often, do
  * not.  No counterpart in the reference. */
 int ob_operand_fence(void* cuda_stream);
 
@@ -311,8 +311,8 @@ int ob_requant_nvfp4(const void* src, int32_t l, int32_t rows, int32_t cols, voi
  * which ob_chain_fp8 / ob_chain_mxfp4 take as ObBatch.x_codes / x_scales.  Strides are in elements: `*_ld` between tokens, `*_hd`
  * between a token's heads (H = 1: unused).  An output may be the same memory as an input of the same strides, else they must not
  * overlap.  A row that holds a NaN has NaN for its y, scales and codes.  One that holds an infinity has NaN there for its y and zeros
- * elsewhere, NaN for its FP8 scale and codes, and MXFP4 blocks of those y.  One launch, capturable, no workspace; M = 0 does nothing.  No counterpart in the reference, which leaves the norm to
- * vLLM (RMSNorm, vllm/model_executor/layers/layernorm.py). */
+ * elsewhere, NaN for its FP8 scale and codes, and MXFP4 blocks of those y.  One launch, capturable, no workspace; M = 0 does nothing.  No
+ * counterpart in the reference, which leaves the norm to vLLM (RMSNorm, vllm/model_executor/layers/layernorm.py). */
 enum { OB_QUANT_NONE = 0, OB_QUANT_FP8 = 1, OB_QUANT_MXFP4 = 2 };
 typedef struct ObRmsNorm {
     int32_t M, H, K;                 /* tokens, heads of a token (1: rows of K), elements of a row; MXFP4: K a multiple of 32 */
